@@ -122,6 +122,19 @@ SIGNATURES = {
     "agpt_b200_embedding_grad": (C.c_int, [vp] * 3 + [i64, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
     "agpt_b200_embedding_grad_serial": (C.c_int, [vp] * 3 + [i64, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
     "agpt_b200_embedding_grad_workspace_bytes": (i64, [i64, C.c_int, C.c_int]),
+    "agpt_b200_embedding_lookup": (C.c_int, [vp, i64, C.c_int, vp, C.c_int, vp, i64, C.c_int, C.c_int, f32, vp]),
+    "agpt_b200_embedding_grad_sorted": (C.c_int, [vp, i64, C.c_int, vp, C.c_int, vp, C.c_int, i64, C.c_int, C.c_int, f32, C.c_int, vp, i64, vp]),
+    "agpt_b200_embedding_grad_sorted_workspace_bytes": (i64, [i64, C.c_int, C.c_int]),
+    "agpt_b200_qk_norm_rope": (C.c_int, [vp, i64, vp, i64, C.c_int, vp, vp, vp, vp, vp, C.c_int, i64, C.c_int, C.c_int, C.c_int, f32, vp, i64, C.c_int,
+                                         vp, i64, C.c_int, vp]),
+    "agpt_b200_qk_norm_rope_backward": (C.c_int, [vp, i64, vp, i64, C.c_int, vp, i64, vp, i64, C.c_int, vp, vp, vp, vp, vp, C.c_int, i64, C.c_int, C.c_int,
+                                                  C.c_int, f32, vp, i64, vp, i64, vp, vp, vp, i64, vp]),
+    "agpt_b200_qk_norm_rope_backward_workspace_bytes": (i64, [C.c_int]),
+    "agpt_b200_act8_pack": (C.c_int, [vp, i64, C.c_int, vp, vp, i64, C.c_int, vp]),
+    "agpt_b200_act8_unpack": (C.c_int, [vp, vp, vp, i64, C.c_int, vp]),
+    "agpt_b200_act8_relu_backward": (C.c_int, [vp, i64, vp, vp, i64, C.c_int, vp]),
+    "agpt_b200_act8_weight_grad": (C.c_int, [vp, vp, vp, i64, i64, C.c_int, C.c_int, vp, vp, vp, i64, vp]),
+    "agpt_b200_act8_weight_grad_workspace_bytes": (i64, [i64, C.c_int, C.c_int]),
     "cuda_adam_bulk": (None, [vp] * 4 + [f32] * 4 + [C.c_int, C.c_int]),
     "cuda_sgd_bulk": (None, [vp, vp, f32, C.c_int]),
     "cuda_momentum_bulk": (None, [vp] * 3 + [f32, f32, C.c_int]),

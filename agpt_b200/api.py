@@ -755,6 +755,244 @@ def embedding_grad(grad, ids32, vocab, out=None, accumulate=False, serial=False)
     return out
 
 
+# rows of float32 or bfloat16, on any device and stream ------------------------------------------------------------------
+def _row_type(t, name, width=None, rows=None):
+    """KV_F32 or KV_BF16 of a 2-D CUDA tensor whose rows are contiguous (a column range of a wider matrix will do)."""
+    import torch
+    if not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.shape[0] and t.stride(1) != 1):
+        raise AgptError(f"{name} must be a 2-D CUDA tensor with contiguous rows")
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise AgptError(f"{name} has dtype {t.dtype}, expected float32 or bfloat16")
+    if (width is not None and t.shape[1] != width) or (rows is not None and t.shape[0] != rows):
+        raise AgptError(f"{name} has shape {tuple(t.shape)}, expected {(rows if rows is not None else t.shape[0], width if width is not None else t.shape[1])}")
+    return KV_BF16 if t.dtype == torch.bfloat16 else KV_F32
+
+
+def _row_stride(t, name):
+    """Elements from a row to the next; rows that share memory (an expanded tensor) are refused for outputs by the library, for inputs here."""
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise AgptError(f"{name} has overlapping rows (stride {ld}): make it contiguous")
+    return ld
+
+
+def _same_device(ref, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise AgptError(f"{name} is on {t.device}, expected {ref.device}")
+
+
+def _flat(t, name, dtype, numel, ref):
+    if t.dtype != dtype or t.device != ref.device or not t.is_contiguous() or t.numel() != numel:
+        raise AgptError(f"{name} must be a contiguous {dtype} tensor of {numel} elements on {ref.device}")
+    return t.data_ptr()
+
+
+def _call(ref, what, fn, *args):
+    """fn(*args, stream) on the device of ref and its current stream."""
+    import torch
+    stream = torch.cuda.current_stream(ref.device).cuda_stream
+    if ref.device.index == torch.cuda.current_device():
+        return check(fn(*args, stream), what)
+    with torch.cuda.device(ref.device):
+        return check(fn(*args, stream), what)
+
+
+def _scratch_of(ref, what, fn, *args):
+    """Workspace of a call: fresh memory of the caching allocator, so that streams and captured graphs never share it."""
+    import torch
+    with torch.cuda.device(ref.device):
+        need = check(fn(*args), what)
+        return torch.empty(max(int(need), 16), dtype=torch.uint8, device=ref.device), int(need)
+
+
+def _ids(ids, n, ref):
+    import torch
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 1 or not ids.is_contiguous() or ids.device != ref.device or (n is not None and ids.numel() != n):
+        raise AgptError(f"ids must be a contiguous 1-D int32 or int64 tensor{'' if n is None else f' of {n} entries'} on {ref.device}")
+    return int(ids.dtype == torch.int64)
+
+
+def embedding_lookup(emb, ids, scale: float = 1.0, out=None):
+    """out[i] = scale * emb[ids[i]] [n, d_model], of the table's type (float32 or bfloat16); a zero row where an id lies outside the table."""
+    import torch
+    kind = _row_type(emb, "emb")
+    vocab, d = emb.shape
+    wide, ld = _ids(ids, None, emb), _row_stride(emb, "emb")
+    n = ids.numel()
+    if out is None:
+        out = torch.empty((n, d), dtype=emb.dtype, device=emb.device)
+    elif _row_type(out, "out", d, n) != kind or not out.is_contiguous() or out.device != emb.device:
+        raise AgptError("out must be a contiguous tensor of the table's type on its device")
+    _call(emb, "embedding_lookup", lib().agpt_b200_embedding_lookup, emb.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), n, d, vocab, scale)
+    return out
+
+
+def embedding_grad_sorted(grad, ids, vocab: int, scale: float = 1.0, out=None, accumulate: bool = False):
+    """Gradient of embedding_lookup's table, [vocab, d_model]: scale times the sum of grad over the rows of each token, summed in float32 in an
+    order that repeats, for vocabularies of any size (embedding_grad keeps tables of up to 400 symbols in shared memory).  out: float32 (the
+    default) or bfloat16, added to with accumulate."""
+    import torch
+    kind = _row_type(grad, "grad")
+    n, d = grad.shape
+    wide, ld = _ids(ids, n, grad), _row_stride(grad, "grad")
+    if out is None:
+        out = (torch.zeros if accumulate else torch.empty)((vocab, d), dtype=torch.float32, device=grad.device)
+    out_kind = _row_type(out, "out", d, vocab)
+    if not out.is_contiguous() or out.device != grad.device:
+        raise AgptError("out must be contiguous and on the device of grad")
+    L = lib()
+    ws, need = _scratch_of(grad, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted_workspace_bytes, n, d, vocab)
+    _call(grad, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted, grad.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), out_kind, n, d, vocab,
+          scale, int(accumulate), ws.data_ptr(), need)
+    return out
+
+
+def _rope_args(q, k, pos, cos, sin, q_gain, k_gain):
+    """Sizes and pointers shared by the two directions of qk_norm_rope."""
+    import torch
+    kind = _row_type(q, "q")
+    n, hd = q.shape[0], cos.shape[-1]
+    if _row_type(k, "k", None, n) != kind:
+        raise AgptError("q and k must have the same dtype")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1:
+        raise AgptError("cos and sin must be [positions, head_dim] tables")
+    if hd < 2 or hd % 2 or hd > 256 or q.shape[1] % hd or k.shape[1] % hd or not q.shape[1] or not k.shape[1]:
+        raise AgptError(f"widths {q.shape[1]} and {k.shape[1]} must be multiples of an even head_dim up to 256, the tables have {hd}")
+    _same_device(q, k=k)
+    tables = [_flat(t, name, torch.float32, t.numel(), q) for name, t in (("cos", cos), ("sin", sin))]
+    at = _flat(pos, "pos", torch.int32, n, q)
+    gains = [None if g is None else _flat(g, name, torch.float32, hd, q) for name, g in (("q_gain", q_gain), ("k_gain", k_gain))]
+    return kind, n, hd, gains + [at] + tables + [cos.shape[0]], [n, q.shape[1] // hd, k.shape[1] // hd, hd]
+
+
+def qk_norm_rope(q, k, q_gain, k_gain, pos, cos, sin, eps: float = 1e-6, k_dtype=None, q_out=None, k_out=None):
+    """Queries and keys with every head normalised by its root mean square (times a gain [head_dim], None: ones) and rotated by its row's
+    position (as rope_pair_ does), in one pass.  q [n, heads * head_dim], k [n, kv_heads * head_dim], float32 or bfloat16, also as column
+    ranges of one matrix; head_dim is the width of the tables.  k_dtype: torch.bfloat16 writes the keys as a bfloat16 store.  Outputs are new
+    tensors, or q_out and k_out (q and k themselves will do).  Returns (q, k)."""
+    import torch
+    kind, n, hd, tab, sizes = _rope_args(q, k, pos, cos, sin, q_gain, k_gain)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k_dtype or k.dtype, device=k.device) if k_out is None else k_out
+    types = _row_type(q_out, "q_out", q.shape[1], n), _row_type(k_out, "k_out", k.shape[1], n)
+    if k_dtype is not None and k_out.dtype != k_dtype:
+        raise AgptError(f"k_out has dtype {k_out.dtype}, k_dtype says {k_dtype}")
+    _same_device(q, q_out=q_out, k_out=k_out)
+    _call(q, "qk_norm_rope", lib().agpt_b200_qk_norm_rope, q.data_ptr(), _row_stride(q, "q"), k.data_ptr(), _row_stride(k, "k"), kind, *tab, *sizes, eps,
+          q_out.data_ptr(), _row_stride(q_out, "q_out"), types[0], k_out.data_ptr(), _row_stride(k_out, "k_out"), types[1])
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq, dk, q, k, q_gain, k_gain, pos, cos, sin, dq_gain=None, dk_gain=None, eps: float = 1e-6, q_out=None, k_out=None):
+    """Gradients of qk_norm_rope with respect to q and k (of their type), from those of its outputs (dq, dk: both float32 or both bfloat16) and
+    its inputs.  dq_gain, dk_gain [head_dim] float32 are accumulated into (None: not wanted).  q_out and k_out may be dq and dk."""
+    import torch
+    kind, n, hd, tab, sizes = _rope_args(q, k, pos, cos, sin, q_gain, k_gain)
+    grad_kind = _row_type(dq, "dq", q.shape[1], n)
+    if _row_type(dk, "dk", k.shape[1], n) != grad_kind:
+        raise AgptError("dq and dk must have the same dtype")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+    if _row_type(q_out, "q_out", q.shape[1], n) != kind or _row_type(k_out, "k_out", k.shape[1], n) != kind:
+        raise AgptError("q_out and k_out must have the dtype of q and k")
+    _same_device(q, dq=dq, dk=dk, q_out=q_out, k_out=k_out)
+    gains = [None if g is None else _flat(g, name, torch.float32, hd, q) for name, g in (("dq_gain", dq_gain), ("dk_gain", dk_gain))]
+    L = lib()
+    ws, need = _scratch_of(q, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward_workspace_bytes, hd)
+    _call(q, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward, dq.data_ptr(), _row_stride(dq, "dq"), dk.data_ptr(), _row_stride(dk, "dk"), grad_kind,
+          q.data_ptr(), _row_stride(q, "q"), k.data_ptr(), _row_stride(k, "k"), kind, *tab, *sizes, eps, q_out.data_ptr(), _row_stride(q_out, "q_out"),
+          k_out.data_ptr(), _row_stride(k_out, "k_out"), *gains, ws.data_ptr(), need)
+    return q_out, k_out
+
+
+class Act8:
+    """An activation [n, cols] kept in 8 bits: codes uint8 [n, cols rounded up to 32] (e4m3) and scales uint8 [blocks of 32 columns, n rounded up to 16];
+    the value of a code is the e4m3 number times 2^(scale - 127), a block of scale 255 is NaN (see agpt_b200_act8_pack)."""
+
+    __slots__ = ("codes", "scales", "cols")
+
+    def __init__(self, codes, scales, cols: int):
+        import torch
+        n, blocks = codes.shape[0], -(-cols // 32)
+        if cols < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device or not codes.is_contiguous() or \
+                not scales.is_contiguous() or tuple(codes.shape) != (n, blocks * 32) or tuple(scales.shape) != (blocks, (n + 15) // 16 * 16):
+            raise AgptError(f"an 8-bit activation of {cols} columns has contiguous uint8 codes [n, {blocks * 32}] and scales [{blocks}, n rounded up to 16]")
+        if not codes.is_cuda or (codes.data_ptr() | scales.data_ptr()) & 15:
+            raise AgptError("codes and scales must be CUDA tensors on 16-byte boundaries")
+        self.codes, self.scales, self.cols = codes, scales, int(cols)
+
+    @property
+    def shape(self):
+        return self.codes.shape[0], self.cols
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def act8_pack(x) -> Act8:
+    """x [n, cols] (float32 or bfloat16) as an 8-bit checkpoint: at most 2^-4 of a value is lost, or half a step of the block's smallest code; what is not
+    zero does not become zero."""
+    import torch
+    kind = _row_type(x, "x")
+    n, cols = x.shape
+    if cols < 1:
+        raise AgptError("x has no columns")
+    blocks = -(-cols // 32)
+    a = Act8(torch.empty((n, blocks * 32), dtype=torch.uint8, device=x.device), torch.empty((blocks, (n + 15) // 16 * 16), dtype=torch.uint8, device=x.device), cols)
+    _call(x, "act8_pack", lib().agpt_b200_act8_pack, x.data_ptr(), _row_stride(x, "x"), kind, a.codes.data_ptr(), a.scales.data_ptr(), n, cols)
+    return a
+
+
+def act8_unpack(a: Act8):
+    """The values of a checkpoint, float32 [n, cols]."""
+    import torch
+    out = torch.empty(a.shape, dtype=torch.float32, device=a.device)
+    _call(out, "act8_unpack", lib().agpt_b200_act8_unpack, a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr(), *a.shape)
+    return out
+
+
+def _act8_grad(a, grad, cols):
+    import torch
+    if _row_type(grad, "grad", cols, a.shape[0]) != KV_F32:
+        raise AgptError("grad must be float32")
+    _same_device(grad, activation=a)
+    return _row_stride(grad, "grad")
+
+
+def act8_relu_backward(grad, a: Act8, out=None):
+    """grad where the kept activation is above 0, else 0: relu_backward with the mask read from a checkpoint.  out may be grad."""
+    import torch
+    ld = _act8_grad(a, grad, a.cols)
+    if out is None:
+        out = torch.empty(grad.shape, dtype=torch.float32, device=grad.device)
+    elif _row_type(out, "out", *grad.shape[::-1]) != KV_F32 or not out.is_contiguous() or out.device != grad.device:
+        raise AgptError("out must be a contiguous float32 tensor of the shape of grad on its device")
+    _call(grad, "act8_relu_backward", lib().agpt_b200_act8_relu_backward, grad.data_ptr(), ld, a.codes.data_ptr(), out.data_ptr(), *a.shape)
+    return out
+
+
+def act8_weight_grad(a: Act8, grad, out=None, bias_grad: bool = True):
+    """(X^T grad [cols of a, cols of grad], column sums of grad): weight and bias gradients of a projection whose input was kept in 8 bits, accurate to
+    float32 over the kept values.  bias_grad=False: (weight gradient, None)."""
+    import torch
+    n, m = a.shape
+    ld, cols = _act8_grad(a, grad, grad.shape[-1]), grad.shape[1]
+    if cols < 1:
+        raise AgptError("grad has no columns")
+    if out is None:
+        out = torch.empty((m, cols), dtype=torch.float32, device=grad.device)
+    elif _row_type(out, "out", cols, m) != KV_F32 or not out.is_contiguous() or out.device != grad.device:
+        raise AgptError(f"out must be a contiguous float32 tensor of shape {(m, cols)} on the device of grad")
+    db = torch.empty(cols, dtype=torch.float32, device=grad.device) if bias_grad else None
+    L = lib()
+    ws, need = _scratch_of(grad, "act8_weight_grad", L.agpt_b200_act8_weight_grad_workspace_bytes, n, m, cols)
+    _call(grad, "act8_weight_grad", L.agpt_b200_act8_weight_grad, a.codes.data_ptr(), a.scales.data_ptr(), grad.data_ptr(), ld, n, m, cols, out.data_ptr(),
+          None if db is None else db.data_ptr(), ws.data_ptr(), need)
+    return out, db
+
+
 OPTIMIZER_KINDS = {"sgd": 0, "momentum": 1, "rmsprop": 2, "adam": 3}
 
 

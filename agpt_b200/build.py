@@ -13,7 +13,8 @@ SOURCES = [os.path.join(HERE, "csrc", "kernels.cu"), os.path.join(HERE, "csrc", 
            os.path.join(HERE, "csrc", "host_trie.cpp"), os.path.join(HERE, "csrc", "trie_suffix.cpp"),
            os.path.join(HERE, "csrc", "trie_gpu.cu"),
            os.path.join(HERE, "csrc", "step_gemm.cu"), os.path.join(HERE, "csrc", "train_step.cu"),
-           os.path.join(HERE, "csrc", "groups.cu")]
+           os.path.join(HERE, "csrc", "groups.cu"),
+           os.path.join(HERE, "csrc", "embedding.cu"), os.path.join(HERE, "csrc", "qk_norm.cu"), os.path.join(HERE, "csrc", "act8.cu")]
 
 
 # The two GEMM translation units instantiate CUTLASS templates, and gemm_sm100.cu re-instantiates the SM100 fast-FP32
@@ -54,7 +55,8 @@ def cutlass_include():
     return None
 
 
-HEADERS = [os.path.join(HERE, "csrc", "internal.h"), os.path.join(HERE, "csrc", "step_gemm.h"), os.path.join(HERE, "csrc", "tc100.cuh"), os.path.join(HERE, "csrc", "pdl.cuh"), os.path.join(HERE, "..", "include", "agpt_b200.h")]
+HEADERS = [os.path.join(HERE, "csrc", "internal.h"), os.path.join(HERE, "csrc", "step_gemm.h"), os.path.join(HERE, "csrc", "tc100.cuh"), os.path.join(HERE, "csrc", "pdl.cuh"),
+           os.path.join(HERE, "csrc", "vec.cuh"), os.path.join(HERE, "..", "include", "agpt_b200.h")]
 
 
 OBJ_DIR = os.path.join(HERE, "_build")

@@ -1,0 +1,586 @@
+// Rows of a token table times a scale, and the gradient of the table summed over equal tokens, for vocabularies of any size.
+//
+//   lookup     out[i] = scale * E[id_i], a zero row where id_i lies outside the vocabulary
+//   gradient   dE[t]  = scale * sum of g[i] over the rows i with id_i = t
+//
+// Both are bound by memory: a gradient reads n rows once.  The sums repeat bit for bit, without atomics on floating values: the rows
+// are ordered by token (a stable counting sort of (token, row) pairs, 8 bytes a row), pieces of the order are summed by warps, and what a
+// token has in several pieces is added in the order of the pieces.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/agpt_b200.h"
+#include "internal.h"
+#include "pdl.cuh"
+#include "vec.cuh"
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+int launch_status(const char *who) {
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    return AGPT_OK;
+}
+
+// the token of row i, or `vocab` where it lies outside the vocabulary
+__device__ __forceinline__ uint32_t token_of(const void *ids, int wide, int64_t i, uint32_t vocab) {
+    if (wide) {
+        const int64_t t = __ldg(reinterpret_cast<const long long *>(ids) + i);
+        return t >= 0 && t < (int64_t)vocab ? (uint32_t)t : vocab;
+    }
+    const uint32_t t = (uint32_t)__ldg(reinterpret_cast<const int *>(ids) + i);
+    return t < vocab ? t : vocab;
+}
+
+// ---- lookup: a group of 2^lanes_log2 lanes per row, LOOK_ROWS rows of it in flight -------------------------------------------------
+constexpr int LOOK_ROWS = 4;
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ emb, int64_t ld, const void *__restrict__ ids, int wide, T *__restrict__ out,
+                                                      int64_t n, int d, uint32_t vocab, float scale, int lanes_log2) {
+    pdl_wait();
+    pdl_next();
+    const int lanes = 1 << lanes_log2, per_block = 256 >> lanes_log2;
+    const int c0 = (threadIdx.x & (lanes - 1)) * VEC;
+    const int64_t r0 = (int64_t)blockIdx.x * per_block * LOOK_ROWS + (threadIdx.x >> lanes_log2);
+    uint32_t id[LOOK_ROWS];
+#pragma unroll
+    for (int u = 0; u < LOOK_ROWS; u++) {
+        const int64_t r = r0 + (int64_t)u * per_block;
+        id[u] = r < n ? token_of(ids, wide, r, vocab) : vocab;
+    }
+    for (int c = c0; c < d; c += lanes * VEC) {
+        float v[LOOK_ROWS][VEC];
+#pragma unroll
+        for (int u = 0; u < LOOK_ROWS; u++) {
+            if (id[u] < vocab) vec::load<VEC>(emb + (int64_t)id[u] * ld + c, v[u]);
+            else
+#pragma unroll
+                for (int i = 0; i < VEC; i++) v[u][i] = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < LOOK_ROWS; u++) {
+            const int64_t r = r0 + (int64_t)u * per_block;
+            if (r >= n) break;
+            if (id[u] < vocab)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) v[u][i] *= scale;
+            vec::store<VEC>(out + r * d + c, v[u]);
+        }
+    }
+}
+
+// ---- order of the rows by token: counting sort, least significant digit first -----------------------------------------------------
+// A pass counts the digits of each block's rows (count_kernel), turns the counts into places over the blocks (place_kernel) and moves
+// the pairs (move_kernel): a warp of a block owns a run of rows and has its own counters, so rows of one digit keep their order.
+constexpr int MOVE_WARPS = 8, DIGIT_BITS_MAX = 11;
+
+template <bool FIRST>
+__device__ __forceinline__ uint32_t key_of(const void *ids, int wide, const uint2 *in, int64_t i, uint32_t vocab) {
+    return FIRST ? token_of(ids, wide, i, vocab) : __ldg(&in[i].x);
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(256) count_kernel(const void *__restrict__ ids, int wide, const uint2 *__restrict__ in, int64_t n, int64_t chunk, uint32_t vocab,
+                                                     int shift, int bins, uint32_t *__restrict__ counts) {
+    pdl_wait();
+    pdl_next();
+    extern __shared__ uint32_t s_hist[];
+    for (int b = threadIdx.x; b < bins; b += 256) s_hist[b] = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)blockIdx.x * chunk, i1 = min(i0 + chunk, n);
+#pragma unroll 4
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) atomicAdd(&s_hist[(key_of<FIRST>(ids, wide, in, i, vocab) >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)blockIdx.x * bins + b] = s_hist[b];
+}
+
+// counts[block][digit] -> rows of the digit in earlier blocks; totals[digit].  A block has 32 digits and eight slices of the blocks.
+__global__ void __launch_bounds__(256) place_kernel(uint32_t *__restrict__ counts, int blocks, int bins, uint32_t *__restrict__ totals) {
+    pdl_wait();
+    pdl_next();
+    __shared__ uint32_t s[8][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
+    const int b0 = blocks * w / 8, b1 = blocks * (w + 1) / 8;
+    uint32_t sum = 0;
+    if (d < bins)
+#pragma unroll 8
+        for (int b = b0; b < b1; b++) sum += counts[(int64_t)b * bins + d];
+    s[w][lane] = sum;
+    __syncthreads();
+    uint32_t at = 0;
+    for (int k = 0; k < w; k++) at += s[k][lane];
+    if (d >= bins) return;
+    if (w == 7) totals[d] = at + sum;
+#pragma unroll 8
+    for (int b = b0; b < b1; b++) {
+        const uint32_t x = counts[(int64_t)b * bins + d];
+        counts[(int64_t)b * bins + d] = at;
+        at += x;
+    }
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__restrict__ ids, int wide, const uint2 *__restrict__ in, int64_t n, int64_t chunk,
+                                                                uint32_t vocab, int shift, int bits, const uint32_t *__restrict__ counts,
+                                                                const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
+    pdl_wait();
+    pdl_next();
+    extern __shared__ uint32_t s_at[];                     // [MOVE_WARPS][bins] counters, then places; [bins] starts of the digits
+    const int bins = 1 << bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    uint32_t *mine = s_at + w * bins, *start = s_at + MOVE_WARPS * bins;
+    __shared__ uint32_t s_warp[MOVE_WARPS];
+    for (int b = threadIdx.x; b < MOVE_WARPS * bins; b += MOVE_WARPS * 32) s_at[b] = 0;
+    // starts of the digits: a thread has bins / 256 neighbours (bins >= 256, or the threads behind have none)
+    const int each = (bins + MOVE_WARPS * 32 - 1) / (MOVE_WARPS * 32);
+    uint32_t sum = 0;
+    for (int k = 0; k < each; k++) {
+        const int b = threadIdx.x * each + k;
+        if (b < bins) sum += __ldg(totals + b);
+    }
+    uint32_t run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += x;
+    }
+    if (lane == 31) s_warp[w] = run;
+    __syncthreads();
+    uint32_t at = run - sum;
+    for (int k = 0; k < w; k++) at += s_warp[k];
+    for (int k = 0; k < each; k++) {
+        const int b = threadIdx.x * each + k;
+        if (b < bins) { start[b] = at; at += __ldg(totals + b); }
+    }
+    // digits of each warp's rows
+    const int64_t own = chunk / MOVE_WARPS, i0 = (int64_t)blockIdx.x * chunk + w * own, i1 = min(i0 + own, n);
+#pragma unroll 4
+    for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[(key_of<FIRST>(ids, wide, in, i, vocab) >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += MOVE_WARPS * 32) {
+        uint32_t t = start[b] + __ldg(counts + (int64_t)blockIdx.x * bins + b);
+#pragma unroll
+        for (int k = 0; k < MOVE_WARPS; k++) {
+            const uint32_t x = s_at[k * bins + b];
+            s_at[k * bins + b] = t;
+            t += x;
+        }
+    }
+    __syncthreads();
+    for (int64_t i = i0; i < i1; i += 32) {
+        const bool live = i + lane < i1;
+        uint2 p = make_uint2(0, 0);
+        if (live) p = FIRST ? make_uint2(token_of(ids, wide, i + lane, vocab), (uint32_t)(i + lane)) : __ldg(in + i + lane);
+        const uint32_t digit = live ? (p.x >> shift) & (bins - 1) : 0xffffffffu;
+        const uint32_t same = __match_any_sync(0xffffffffu, digit);
+        uint32_t to = 0;
+        if (live) to = mine[digit] + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (live) {
+            if (lane == 31 - __clz(same)) mine[digit] = to + 1;      // the last of them
+            out[to] = p;
+        }
+        __syncwarp();
+    }
+}
+
+// ---- sums over the ordered rows ----------------------------------------------------------------------------------------------------
+// A warp has `run` places of the order and 32 * VEC columns, a block SUM_WARPS warps side by side.  Tokens that end where they began are
+// written; the warps' first and last sums meet in shared memory; what a block has of a token that began before it goes to head[block], of
+// one that goes on behind it to tail[block], and join_kernel adds tail and heads in order.
+constexpr int SUM_WARPS = 8, FILL_TOKENS = 64;
+
+template <typename O, int VEC>
+__device__ __forceinline__ void write_row(O *out, int64_t at, float (&v)[VEC], float scale, int accumulate) {
+    if (accumulate) {
+        float old[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) old[i] = (float)out[at + i];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = old[i] + scale * v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] *= scale;
+    }
+    vec::store<VEC>(out + at, v);
+}
+
+// zero rows of the tokens that no row has
+template <typename O>
+__device__ void fill_absent(const uint2 *order, int64_t n, O *out, int d, uint32_t vocab, int64_t first) {
+    __shared__ uint32_t s_absent[FILL_TOKENS / 32];
+    if (threadIdx.x < FILL_TOKENS) {
+        const int64_t t = first + threadIdx.x;
+        bool absent = false;
+        if (t < vocab) {
+            int64_t lo = 0, hi = n;
+            while (lo < hi) {
+                const int64_t mid = (lo + hi) >> 1;
+                if (__ldg(&order[mid].x) < (uint32_t)t) lo = mid + 1; else hi = mid;
+            }
+            absent = lo >= n || __ldg(&order[lo].x) != (uint32_t)t;
+        }
+        const uint32_t b = __ballot_sync(0xffffffffu, absent);
+        if ((threadIdx.x & 31) == 0) s_absent[threadIdx.x >> 5] = b;
+    }
+    __syncthreads();
+    const bool wide = (d * sizeof(O)) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    for (int k = threadIdx.x >> 5; k < FILL_TOKENS; k += blockDim.x >> 5) {
+        if (!(s_absent[k >> 5] >> (k & 31) & 1)) continue;
+        O *row = out + (first + k) * (int64_t)d;
+        if (wide)
+            for (int c = threadIdx.x & 31; c < (int)(d * sizeof(O) / 16); c += 32) reinterpret_cast<uint4 *>(row)[c] = make_uint4(0, 0, 0, 0);
+        else
+            for (int c = threadIdx.x & 31; c < d; c += 32) row[c] = (O)0.f;
+    }
+}
+
+template <typename T, typename O, int VEC>
+__global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict__ grad, int64_t ld, const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab,
+                                                              int run, int64_t blocks, float scale, int accumulate, O *__restrict__ out, float *__restrict__ head,
+                                                              float *__restrict__ tail) {
+    pdl_wait();
+    pdl_next();
+    constexpr int COLS = 32 * VEC, U = 8;
+    __shared__ float s_part[SUM_WARPS][2][COLS];
+    __shared__ uint32_t s_first[SUM_WARPS], s_last[SUM_WARPS];
+    __shared__ uint8_t s_in[SUM_WARPS], s_out[SUM_WARPS], s_through[SUM_WARPS];
+    if (blockIdx.x >= blocks) {
+        if (blockIdx.y == 0) fill_absent(order, n, out, d, vocab, (blockIdx.x - blocks) * FILL_TOKENS);
+        return;
+    }
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * COLS + lane * VEC;
+    const int64_t p0 = ((int64_t)blockIdx.x * SUM_WARPS + w) * run, p1 = min(p0 + run, n);
+    if (p0 < n) {
+        float acc[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) acc[i] = 0.f;
+        const uint32_t first = __ldg(&order[p0].x), last = __ldg(&order[p1 - 1].x);
+        const bool in = p0 > 0 && __ldg(&order[p0 - 1].x) == first, goes_on = p1 < n && __ldg(&order[p1].x) == last;
+        uint32_t cur = first;
+        bool begun_before = in;
+        for (int64_t p = p0; p < p1; p += 32) {
+            const uint2 mine = p + lane < p1 ? __ldg(order + p + lane) : make_uint2(vocab, 0);
+            const int live = (int)min((int64_t)32, p1 - p);
+            for (int k0 = 0; k0 < live; k0 += U) {
+                float v[U][VEC];
+                uint32_t key[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    key[u] = __shfl_sync(0xffffffffu, mine.x, k0 + u);
+                    const uint32_t row = __shfl_sync(0xffffffffu, mine.y, k0 + u);
+                    if (k0 + u < live && key[u] < vocab && c < d) vec::load<VEC>(grad + (int64_t)row * ld + c, v[u]);
+                    else
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) v[u][i] = 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (k0 + u >= live) break;
+                    if (key[u] != cur) {
+                        if (begun_before) {
+#pragma unroll
+                            for (int i = 0; i < VEC; i++) s_part[w][0][lane * VEC + i] = acc[i];
+                        } else if (cur < vocab && c < d) write_row<O, VEC>(out, (int64_t)cur * d + c, acc, scale, accumulate);
+                        cur = key[u];
+                        begun_before = false;
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) acc[i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) acc[i] += v[u][i];
+                }
+            }
+        }
+        if (begun_before || goes_on) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) s_part[w][begun_before ? 0 : 1][lane * VEC + i] = acc[i];
+        } else if (cur < vocab && c < d) write_row<O, VEC>(out, (int64_t)cur * d + c, acc, scale, accumulate);
+        if (lane == 0) {
+            s_first[w] = first; s_last[w] = last;
+            s_in[w] = in; s_out[w] = goes_on; s_through[w] = begun_before && goes_on;
+        }
+    }
+    __syncthreads();
+    // the warps in order; a thread has a column
+    const int64_t b0 = (int64_t)blockIdx.x * SUM_WARPS * run;
+    const int warps = (int)min((int64_t)SUM_WARPS, (n - b0 + run - 1) / run);
+    for (int k = threadIdx.x; k < COLS; k += SUM_WARPS * 32) {
+        const int col = blockIdx.y * COLS + k;
+        if (col >= d) break;
+        float acc = 0.f;
+        bool open = false, before = false;
+        for (int i = 0; i < warps; i++) {
+            if (s_in[i]) {
+                if (!open) { open = before = true; acc = 0.f; }           // the block before had its beginning
+                acc += s_part[i][0][k];
+                if (s_through[i]) continue;
+                if (before) head[(int64_t)blockIdx.x * d + col] = acc;
+                else if (s_first[i] < vocab) {
+                    float one[1] = {acc};
+                    write_row<O, 1>(out, (int64_t)s_first[i] * d + col, one, scale, accumulate);
+                }
+                open = false;
+            }
+            if (s_out[i]) { open = true; before = false; acc = s_part[i][1][k]; }
+        }
+        if (open) (before ? head : tail)[(int64_t)blockIdx.x * d + col] = acc;
+    }
+}
+
+// Tokens that began in this block and go on behind it: tail, then the heads of the blocks that begin with the token.  The heads are cut into
+// as many runs as there are warps.
+template <typename O>
+__global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab, int64_t span, float scale, int accumulate,
+                                                    O *__restrict__ out, const float *__restrict__ head, const float *__restrict__ tail) {
+    pdl_wait();
+    pdl_next();
+    __shared__ float s_part[8][32];
+    __shared__ int64_t s_heads;
+    const int64_t p0 = (int64_t)blockIdx.x * span, p1 = p0 + span;         // the last block has nothing behind it and is not launched
+    const uint32_t key = __ldg(&order[p1 - 1].x);
+    if (key >= vocab || __ldg(&order[p1].x) != key) return;
+    if (p0 > 0 && __ldg(&order[p0].x) == key && __ldg(&order[p0 - 1].x) == key) return;      // began before
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if (w == 0) {
+        int64_t heads = 1;
+        for (bool more = true; more; ) {
+            const int64_t p = p1 + (heads + lane) * span;
+            const uint32_t b = __ballot_sync(0xffffffffu, p < n && __ldg(&order[p].x) == key);
+            heads += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
+            more = b == 0xffffffffu;
+        }
+        if (lane == 0) s_heads = heads;
+    }
+    __syncthreads();
+    const int64_t heads = s_heads, h0 = heads * w / 8, h1 = heads * (w + 1) / 8;
+    for (int c0 = blockIdx.y * 32; c0 < d; c0 += gridDim.y * 32) {
+        const int c = c0 + lane;
+        float acc = 0.f;
+        if (c < d) {
+            if (w == 0) acc = tail[(int64_t)blockIdx.x * d + c];
+#pragma unroll 8
+            for (int64_t h = h0; h < h1; h++) acc += head[(blockIdx.x + 1 + h) * d + c];
+        }
+        s_part[w][lane] = acc;
+        __syncthreads();
+        if (w == 0 && c < d) {
+            for (int k = 1; k < 8; k++) acc += s_part[k][lane];
+            float one[1] = {acc};
+            write_row<O, 1>(out, (int64_t)key * d + c, one, scale, accumulate);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- few rows: one launch, no order -------------------------------------------------------------------------------------------------
+// Every block reads all tokens; the block of a token's first row adds its rows, a run of the rows per warp; blocks behind fill absent tokens.
+constexpr int FEW_ROWS = 512;
+template <typename T, typename O, int VEC>
+__global__ void __launch_bounds__(256) few_rows_kernel(const T *__restrict__ grad, int64_t ld, const void *__restrict__ ids, int wide, int n, int d, uint32_t vocab,
+                                                        float scale, int accumulate, O *__restrict__ out) {
+    pdl_wait();
+    pdl_next();
+    constexpr int COLS = 32 * VEC;
+    __shared__ uint32_t s_id[FEW_ROWS];
+    __shared__ float s_part[8][COLS];
+    __shared__ uint32_t s_present[FILL_TOKENS / 32];
+    for (int i = threadIdx.x; i < n; i += 256) s_id[i] = token_of(ids, wide, i, vocab);
+    if (threadIdx.x < FILL_TOKENS / 32) s_present[threadIdx.x] = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if ((int)blockIdx.x >= n) {
+        const int64_t first = (int64_t)(blockIdx.x - n) * FILL_TOKENS;
+        if (blockIdx.y) return;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const int64_t k = (int64_t)s_id[i] - first;
+            if (k >= 0 && k < FILL_TOKENS) atomicOr(&s_present[k >> 5], 1u << (k & 31));
+        }
+        __syncthreads();
+        for (int k = w; k < FILL_TOKENS && first + k < vocab; k += 8) {
+            if (s_present[k >> 5] >> (k & 31) & 1) continue;
+            for (int c = lane; c < d; c += 32) out[(first + k) * d + c] = (O)0.f;
+        }
+        return;
+    }
+    const int self = blockIdx.x;
+    const uint32_t id = s_id[self];
+    if (id >= vocab) return;
+    int earlier = 0;
+    for (int i = threadIdx.x; i < self; i += 256) earlier |= s_id[i] == id;
+    if (__syncthreads_or(earlier)) return;
+    const int c = blockIdx.y * COLS + lane * VEC, left = n - self;
+    const int i0 = self + left * w / 8, i1 = self + left * (w + 1) / 8;
+    float acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; k++) acc[k] = 0.f;
+    for (int i = i0; i < i1; i += 32) {
+        uint32_t hit = __ballot_sync(0xffffffffu, i + lane < i1 && s_id[i + lane] == id);
+        while (hit) {
+            float v[4][VEC];
+            bool have[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                have[u] = hit != 0;
+                if (have[u] && c < d) vec::load<VEC>(grad + (int64_t)(i + __ffs(hit) - 1) * ld + c, v[u]);
+                hit &= hit - 1;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (have[u] && c < d)
+#pragma unroll
+                    for (int k = 0; k < VEC; k++) acc[k] += v[u][k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; k++) s_part[w][lane * VEC + k] = acc[k];
+    __syncthreads();
+    for (int k = threadIdx.x; k < COLS; k += 256) {
+        const int col = blockIdx.y * COLS + k;
+        if (col >= d) break;
+        float one[1] = {0.f};
+        for (int i = 0; i < 8; i++) one[0] += s_part[i][k];
+        write_row<O, 1>(out, (int64_t)id * d + col, one, scale, accumulate);
+    }
+}
+
+// ---- sizes ----------------------------------------------------------------------------------------------------------------------------
+struct Sizes {
+    int passes, bits;              // of the sort; digits of `bits`
+    int64_t chunk, chunks;         // rows of a block of the sort
+    int run;                       // places of a warp of the sums
+    int64_t blocks;                // of the sums
+    int64_t at_pairs, at_counts, at_totals, at_head, at_tail, bytes;
+};
+Sizes sizes_of(int64_t n, int d, int64_t vocab) {
+    Sizes z;
+    int bits = 0;
+    while ((vocab >> bits) > 0) bits++;                       // keys 0 .. vocab
+    z.passes = (bits + DIGIT_BITS_MAX - 1) / DIGIT_BITS_MAX;
+    z.bits = (bits + z.passes - 1) / z.passes;
+    const int64_t sms = vec::sm_count();
+    z.chunk = (n + 2 * sms - 1) / (2 * sms);
+    z.chunk = z.chunk < 1024 ? 1024 : (z.chunk + 255) / 256 * 256;
+    z.chunks = (n + z.chunk - 1) / z.chunk;
+    z.run = 64;
+    while (z.run > 8 && (n + SUM_WARPS * z.run - 1) / (SUM_WARPS * z.run) * ((d + 127) / 128) < 8 * sms) z.run /= 2;
+    z.blocks = (n + SUM_WARPS * z.run - 1) / (SUM_WARPS * z.run);
+    const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+    z.at_pairs = 0;
+    z.at_counts = up(n * 8 * (z.passes > 1 ? 2 : 1));
+    z.at_totals = z.at_counts + up(z.chunks * (4ll << z.bits));
+    z.at_head = z.at_totals + up(4ll << z.bits);
+    z.at_tail = z.at_head + up(z.blocks * d * 4);
+    z.bytes = z.at_tail + up(z.blocks * d * 4);
+    return z;
+}
+
+template <bool FIRST>
+int sort_pass(const void *ids, int wide, const uint2 *in, int64_t n, const Sizes &z, uint32_t vocab, int pass, char *ws, uint2 *out, cudaStream_t st) {
+    const int bins = 1 << z.bits, shift = pass * z.bits;
+    uint32_t *counts = (uint32_t *)(ws + z.at_counts), *totals = (uint32_t *)(ws + z.at_totals);
+    const size_t smem = (size_t)(MOVE_WARPS + 1) * bins * 4;
+    static bool set[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !set[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(move_kernel<FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (MOVE_WARPS + 1) * 4 << DIGIT_BITS_MAX);
+        if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "embedding_grad_sorted: %s", cudaGetErrorString(e));
+        if (dev >= 0 && dev < 64) set[dev] = true;
+    }
+    pdl_launch(count_kernel<FIRST>, (unsigned)z.chunks, 256, (size_t)bins * 4, st, ids, wide, in, n, z.chunk, vocab, shift, bins, counts);
+    pdl_launch(place_kernel, (unsigned)((bins + 31) / 32), 256, 0, st, counts, (int)z.chunks, bins, totals);
+    pdl_launch(move_kernel<FIRST>, (unsigned)z.chunks, MOVE_WARPS * 32, smem, st, ids, wide, in, n, z.chunk, vocab, shift, z.bits, (const uint32_t *)counts,
+               (const uint32_t *)totals, out);
+    return AGPT_OK;
+}
+
+template <typename T, typename O, int VEC>
+int grad_sorted(const T *grad, int64_t ld, const void *ids, int wide, O *out, int64_t n, int d, uint32_t vocab, float scale, int accumulate, char *ws, cudaStream_t st) {
+    const unsigned slices = (unsigned)((d + 32 * VEC - 1) / (32 * VEC));
+    const int64_t fill = accumulate ? 0 : ((int64_t)vocab + FILL_TOKENS - 1) / FILL_TOKENS;
+    if (n <= FEW_ROWS) {
+        if (n + fill) pdl_launch(few_rows_kernel<T, O, VEC>, dim3((unsigned)(n + fill), slices), 256, 0, st, grad, ld, ids, wide, (int)n, d, vocab, scale, accumulate, out);
+        return launch_status("embedding_grad_sorted");
+    }
+    const Sizes z = sizes_of(n, d, vocab);
+    uint2 *pairs[2] = {(uint2 *)(ws + z.at_pairs), (uint2 *)(ws + z.at_pairs) + n};
+    if (int rc = sort_pass<true>(ids, wide, nullptr, n, z, vocab, 0, ws, pairs[0], st)) return rc;
+    for (int p = 1; p < z.passes; p++)
+        if (int rc = sort_pass<false>(nullptr, 0, pairs[(p - 1) & 1], n, z, vocab, p, ws, pairs[p & 1], st)) return rc;
+    const uint2 *order = pairs[(z.passes - 1) & 1];
+    float *head = (float *)(ws + z.at_head), *tail = (float *)(ws + z.at_tail);
+    pdl_launch(sum_kernel<T, O, VEC>, dim3((unsigned)(z.blocks + fill), slices), SUM_WARPS * 32, 0, st, grad, ld, order, n, d, vocab, z.run, z.blocks, scale, accumulate,
+               out, head, tail);
+    if (z.blocks > 1)
+        pdl_launch(join_kernel<O>, dim3((unsigned)(z.blocks - 1), (unsigned)((d + 31) / 32)), 256, 0, st, order, n, d, vocab, (int64_t)SUM_WARPS * z.run, scale, accumulate,
+                   out, (const float *)head, (const float *)tail);
+    return launch_status("embedding_grad_sorted");
+}
+
+template <typename T>
+int lookup(const T *emb, int64_t ld, const void *ids, int wide, T *out, int64_t n, int d, uint32_t vocab, float scale, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    const bool whole = d % V == 0 && ld % V == 0 && vec::aligned(emb, 16) && vec::aligned(out, 16);
+    const int pieces = whole ? d / V : d;
+    int log2 = 0;
+    while (log2 < 5 && (1 << log2) < pieces) log2++;
+    const int64_t per_block = (256 >> log2) * LOOK_ROWS;
+    const unsigned blocks = (unsigned)((n + per_block - 1) / per_block);
+    if (whole) pdl_launch(lookup_kernel<T, V>, blocks, 256, 0, st, emb, ld, ids, wide, out, n, d, vocab, scale, log2);
+    else pdl_launch(lookup_kernel<T, 1>, blocks, 256, 0, st, emb, ld, ids, wide, out, n, d, vocab, scale, log2);
+    return launch_status("embedding_lookup");
+}
+
+template <typename T>
+int grad_by_output(const T *grad, int64_t ld, const void *ids, int wide, void *out, int out_type, int64_t n, int d, uint32_t vocab, float scale, int accumulate, char *ws,
+                   cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    // whole pieces: both the rows and, written by the same lanes, the table lie on 16-byte boundaries
+    const bool whole = d % V == 0 && ld % V == 0 && vec::aligned(grad, 16) && vec::aligned(out, 16);
+    if (out_type == AGPT_KV_BF16)
+        return whole ? grad_sorted<T, bf16, V>(grad, ld, ids, wide, (bf16 *)out, n, d, vocab, scale, accumulate, ws, st)
+                     : grad_sorted<T, bf16, 1>(grad, ld, ids, wide, (bf16 *)out, n, d, vocab, scale, accumulate, ws, st);
+    return whole ? grad_sorted<T, float, V>(grad, ld, ids, wide, (float *)out, n, d, vocab, scale, accumulate, ws, st)
+                 : grad_sorted<T, float, 1>(grad, ld, ids, wide, (float *)out, n, d, vocab, scale, accumulate, ws, st);
+}
+
+int check_sizes(const char *who, int64_t n, int d, int64_t ld, int64_t vocab, int type) {
+    if (n < 0 || d <= 0 || vocab <= 0 || ld < d) return agpt_set_error(AGPT_E_ARG, "%s: bad argument", who);
+    if (type != AGPT_KV_F32 && type != AGPT_KV_BF16) return agpt_set_error(AGPT_E_ARG, "%s: rows are float32 (0) or bfloat16 (1)", who);
+    if (n > INT32_MAX - 65536 || vocab > INT32_MAX - 65536 || d > 1 << 20) return agpt_set_error(AGPT_E_LIMIT, "%s: more than 2^31 rows or symbols, or 2^20 columns", who);
+    return AGPT_OK;
+}
+
+}  // namespace
+
+extern "C" int agpt_b200_embedding_lookup(const void *d_emb, int64_t emb_ld, int type, const void *d_ids, int ids64, void *d_out, int64_t n, int d_model, int vocab,
+                                          float scale, void *stream) {
+    if (int rc = check_sizes("embedding_lookup", n, d_model, emb_ld, vocab, type)) return rc;
+    if (n == 0) return AGPT_OK;
+    if (!d_emb || !d_ids || !d_out) return agpt_set_error(AGPT_E_ARG, "embedding_lookup: bad argument");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (type == AGPT_KV_BF16) return lookup((const bf16 *)d_emb, emb_ld, d_ids, ids64, (bf16 *)d_out, n, d_model, (uint32_t)vocab, scale, st);
+    return lookup((const float *)d_emb, emb_ld, d_ids, ids64, (float *)d_out, n, d_model, (uint32_t)vocab, scale, st);
+}
+
+extern "C" int64_t agpt_b200_embedding_grad_sorted_workspace_bytes(int64_t n, int d_model, int vocab) {
+    if (int rc = check_sizes("embedding_grad_sorted_workspace_bytes", n, d_model, d_model, vocab, AGPT_KV_F32)) return rc;
+    return n <= FEW_ROWS ? 0 : sizes_of(n, d_model, vocab).bytes;
+}
+
+extern "C" int agpt_b200_embedding_grad_sorted(const void *d_grad, int64_t grad_ld, int type, const void *d_ids, int ids64, void *d_emb_grad, int out_type, int64_t n,
+                                               int d_model, int vocab, float scale, int accumulate, void *d_workspace, int64_t workspace_bytes, void *stream) {
+    if (int rc = check_sizes("embedding_grad_sorted", n, d_model, grad_ld, vocab, type)) return rc;
+    if (out_type != AGPT_KV_F32 && out_type != AGPT_KV_BF16) return agpt_set_error(AGPT_E_ARG, "embedding_grad_sorted: the table's gradient is float32 (0) or bfloat16 (1)");
+    if (!d_emb_grad || (n && (!d_grad || !d_ids))) return agpt_set_error(AGPT_E_ARG, "embedding_grad_sorted: bad argument");
+    const int64_t need = n <= FEW_ROWS ? 0 : sizes_of(n, d_model, vocab).bytes;
+    if (need && (!d_workspace || workspace_bytes < need || !vec::aligned(d_workspace, 16)))
+        return agpt_set_error(AGPT_E_ARG, "embedding_grad_sorted: workspace too small (agpt_b200_embedding_grad_sorted_workspace_bytes)");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (type == AGPT_KV_BF16)
+        return grad_by_output((const bf16 *)d_grad, grad_ld, d_ids, ids64, d_emb_grad, out_type, n, d_model, (uint32_t)vocab, scale, accumulate, (char *)d_workspace, st);
+    return grad_by_output((const float *)d_grad, grad_ld, d_ids, ids64, d_emb_grad, out_type, n, d_model, (uint32_t)vocab, scale, accumulate, (char *)d_workspace, st);
+}

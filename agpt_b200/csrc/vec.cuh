@@ -1,0 +1,81 @@
+// Accesses shared by the row operators whose rows are float32 or bfloat16: a piece of a row as floats, and back.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace vec {
+
+// VEC neighbouring elements, VEC > 1 by one access of their size (16 bytes where a lane takes float4 or eight bfloat16)
+template <int VEC> __device__ __forceinline__ void load(const float *p, float (&v)[VEC]) {
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 x = __ldcs(reinterpret_cast<const float4 *>(p + i));
+            v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = __ldcs(p + i);
+    }
+}
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+template <int VEC> __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&v)[VEC]) {
+    if constexpr (VEC == 8) {
+        const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p));
+        v[0] = low(x.x); v[1] = high(x.x); v[2] = low(x.y); v[3] = high(x.y);
+        v[4] = low(x.z); v[5] = high(x.z); v[6] = low(x.w); v[7] = high(x.w);
+    } else if constexpr (VEC == 4) {
+        const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(p));
+        v[0] = low(x.x); v[1] = high(x.x); v[2] = low(x.y); v[3] = high(x.y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = __bfloat162float(p[i]);
+    }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <int VEC> __device__ __forceinline__ void store(float *p, const float (&v)[VEC]) {
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) reinterpret_cast<float4 *>(p)[i / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) p[i] = v[i];
+    }
+}
+// one rounding to bfloat16, to nearest, of the float32 result
+template <int VEC> __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 8) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+    } else if constexpr (VEC == 4) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) p[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+
+inline bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
+// Division of 64-bit task numbers by a launch constant: the upper half of a product with ceil(2^64 / d), exact while task * d < 2^64
+struct Divide {
+    uint64_t m;
+    explicit Divide(uint32_t d) : m(d > 1 ? ~0ull / d + 1 : 0) {}
+};
+__device__ __forceinline__ int64_t quotient(int64_t a, Divide d) { return d.m ? (int64_t)__umul64hi((uint64_t)a, d.m) : a; }
+
+inline int sm_count() {
+    static int n[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 148;
+    if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
+    return n[dev] > 0 ? n[dev] : 148;
+}
+
+}  // namespace vec

@@ -382,6 +382,55 @@ int agpt_b200_embedding_grad_serial(const float *d_grad, const int32_t *d_ids, f
                                     int vocab, int accumulate, void *d_workspace, int64_t workspace_bytes, void *stream);
 int64_t agpt_b200_embedding_grad_workspace_bytes(int64_t n, int d_model, int vocab);
 
+/* Token tables of any vocabulary, with a scale and in float32 or bfloat16 (no counterpart in the reference beyond its gather and scatter-add).
+ * Types are AGPT_KV_F32 / AGPT_KV_BF16; row strides (`_ld`) count elements.  ids: int32, or int64 with ids64 != 0; an id outside
+ * [0, vocab) gives a zero row and no gradient.
+ *   embedding_lookup       out[i] = scale * emb[ids[i]] (contiguous rows of the table's type; the product in float32, rounded once)
+ *   embedding_grad_sorted  emb_grad[t] = (accumulate ? emb_grad[t] : 0) + scale * sum of grad[i] over the rows with ids[i] == t, summed in float32;
+ *                          every row of the table is written, those of absent tokens with zeros (accumulate: left as they are).  The rows are ordered
+ *                          by token first, so the result repeats bit for bit.  Up to 2^31 rows and symbols. */
+int agpt_b200_embedding_lookup(const void *d_emb, int64_t emb_ld, int type, const void *d_ids, int ids64, void *d_out, int64_t n, int d_model,
+                               int vocab, float scale, void *stream);
+int agpt_b200_embedding_grad_sorted(const void *d_grad, int64_t grad_ld, int type, const void *d_ids, int ids64, void *d_emb_grad, int out_type,
+                                    int64_t n, int d_model, int vocab, float scale, int accumulate, void *d_workspace, int64_t workspace_bytes,
+                                    void *stream);
+int64_t agpt_b200_embedding_grad_sorted_workspace_bytes(int64_t n, int d_model, int vocab);
+
+/* RMS norm per head of queries and keys with their rotation, in one pass:  y = R(pos) (gain * x / sqrt(mean(x^2) + eps))  for each of the q_heads
+ * and k_heads heads of head_dim columns (even, up to 256), rotated as agpt_b200_rope does by tables [n_pos, head_dim] of cos and sin; a position outside the
+ * tables takes the nearest row.  q and k: rows of `type`, their own strides (columns of one projection's output will do); outputs of any of the two types, so
+ * that keys can go straight into a bfloat16 store; an output may be its input where types and strides are equal.  Gains [head_dim] float32, NULL: ones.
+ * eps must be above 0.
+ * Backward: from dq, dk of grad_type and the forward's inputs, the gradients with respect to q and k (of their type; may be written over dq and dk of that type
+ * and stride).  Gain gradients [head_dim] float32 are accumulated into in a fixed order (NULL: not wanted; with both NULL no workspace is needed). */
+int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void *d_k, int64_t k_ld, int type, const float *d_q_gain, const float *d_k_gain,
+                           const int32_t *d_pos, const float *d_cos, const float *d_sin, int n_pos, int64_t n, int q_heads, int k_heads,
+                           int head_dim, float eps, void *d_q_out, int64_t q_out_ld, int q_out_type, void *d_k_out, int64_t k_out_ld,
+                           int k_out_type, void *stream);
+int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, const void *d_dk, int64_t dk_ld, int grad_type, const void *d_q, int64_t q_ld,
+                                    const void *d_k, int64_t k_ld, int type, const float *d_q_gain, const float *d_k_gain, const int32_t *d_pos,
+                                    const float *d_cos, const float *d_sin, int n_pos, int64_t n, int q_heads, int k_heads, int head_dim,
+                                    float eps, void *d_q_out, int64_t q_out_ld, void *d_k_out, int64_t k_out_ld, float *d_q_gain_grad,
+                                    float *d_k_gain_grad, void *d_workspace, int64_t workspace_bytes, void *stream);
+int64_t agpt_b200_qk_norm_rope_backward_workspace_bytes(int head_dim);
+
+/* Activations kept in 8 bits for the backward.  A block is 32 neighbouring columns of a row; it is kept as a scale byte s, which stands for 2^(s - 127), and
+ * 32 codes e4m3.  The scale is the smallest power of two with max |x| <= 448 of it (2^-110 at least), a code x / scale rounded to nearest, ties to even; a value
+ * that is not zero keeps its sign and the smallest code at least, so that the mask of a ReLU is the mask of the codes.  A block with infinity or NaN is NaN as a
+ * whole (scale byte 255, codes 0x7f).
+ *   codes   uint8 [n][cols rounded up to 32], zeros behind the last column;  scales  uint8 [blocks of 32 columns][n rounded up to 16];
+ *           both start on 16-byte boundaries
+ * act8_pack: x of `type`, rows ld elements apart.  act8_unpack: the values, float32 [n, cols].  act8_relu_backward: out = grad where the kept activation is
+ * above 0, else 0 (out contiguous, may be grad itself if that is).  act8_weight_grad: for kept inputs [n, m] of a projection and the gradient [n, cols] of its
+ * output, weight_grad [m, cols] = X^T grad and bias_grad [cols] = column sums of grad (NULL: not wanted), float32-accurate over the kept values and repeatable
+ * bit for bit. */
+int agpt_b200_act8_pack(const void *d_x, int64_t ld, int type, uint8_t *d_codes, uint8_t *d_scales, int64_t n, int cols, void *stream);
+int agpt_b200_act8_unpack(const uint8_t *d_codes, const uint8_t *d_scales, float *d_out, int64_t n, int cols, void *stream);
+int agpt_b200_act8_relu_backward(const float *d_grad, int64_t ld, const uint8_t *d_codes, float *d_out, int64_t n, int cols, void *stream);
+int agpt_b200_act8_weight_grad(const uint8_t *d_codes, const uint8_t *d_scales, const float *d_grad, int64_t ld, int64_t n, int m, int cols,
+                               float *d_weight_grad, float *d_bias_grad, void *d_workspace, int64_t workspace_bytes, void *stream);
+int64_t agpt_b200_act8_weight_grad_workspace_bytes(int64_t n, int m, int cols);
+
 /* Replace the optimizer kernels of the reference's kernel dependency (declared src/cuda/agpt_train.cu:64-72;
  * called in the order clip, update, decay at :5135-5162 and :5190-5214).  The dependency's source is not part of
  * the reference; the rules implemented are
