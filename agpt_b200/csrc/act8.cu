@@ -12,11 +12,13 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/agpt_b200.h"
 #include "internal.h"
 #include "pdl.cuh"
+#include "tc100.cuh"
 #include "vec.cuh"
 
 namespace {
@@ -169,49 +171,275 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 }
 
 // ---- weight gradient: dW[m][N] = X^T G, db[N] = column sums of G ----------------------------------------------------------------------
-// A block has 64 x 64 of dW and a slice of the rows; partial sums are added in slice order.
-constexpr int WG_TILE = 64, WG_ROWS = 32;
-__global__ void __launch_bounds__(256) weight_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t pitch, int blocks,
-                                                      const float *__restrict__ grad, int64_t ld, int64_t n, int m, int cols, int64_t chunk, float *__restrict__ part,
-                                                      float *__restrict__ col_part) {
+// On tcgen05, float32-accurate: a kept value is exact in bfloat16, an element of G is the exact sum of three, so a product is three MMAs.  The MMA's rows are
+// 128 columns of G: a converting thread owns one, walks down the rows and writes its packed pairs to tensor memory.  Up to 256 columns of X, n contiguous, come
+// through shared memory, so that a split of G serves all of them.  Loads are asynchronous copies of 4 (G) and 16 bytes (X) into places that only the copying
+// thread reads again: no alignment is asked of G, and no barrier stands between a copy and its use.  An accumulator leaves tensor memory after every 64 rows
+// and is added in registers (tensor cores truncate when they add).  Blocks own (G tile, X columns, slice of the rows); slices are added in order.
+constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
+constexpr int WG_THREADS = 640;                        // four warps that issue MMAs, four on G, four on X, two groups of four that own an accumulator
+constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 128 * 8, PLANE = WG_ROWS * WG_X * 2;
+constexpr uint32_t OFF_X = RAW_STAGES * RAW_G, OFF_S = OFF_X + RAW_STAGES * RAW_X, OFF_P = OFF_S + RAW_STAGES * RAW_S, OFF_BAR = OFF_P + 2 * PLANE;
+constexpr size_t WG_SMEM = OFF_BAR + 128 + 1024;
+static_assert(WG_SMEM <= 232448 && OFF_P % 1024 == 0, "shared memory");
+constexpr int ACC_COLS = 128, G_COLS = 96, TMEM_COLS = 512;
+constexpr int REG_ISSUE = 40, REG_G = 72, REG_X = 64, REG_ACC = 152;
+static_assert(REG_ISSUE + REG_G + REG_X + 2 * REG_ACC <= 5 * 96, "setmaxnreg draws on the registers of the launch");
+
+struct WeightGrad {
+    const uint8_t *codes, *scales;
+    const float *grad;
+    float *part, *col_part;            // [slices][m][cols], [slices][cols]: the results themselves if there is one slice
+    int64_t ld, n, row_blocks, pitch;
+    int m, cols, code_pitch, slices, x_cols, x_groups, g_tiles;
+    int *status;
+};
+
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+// Two codes (bytes lo, lo + 1 of w) as bfloat16 values times 2^(scale - 127).  Sign, exponent and fraction of a code moved to their places in a bfloat16 make its
+// value times 2^-120, subnormal ones included; f = 2^(scale - 7), and for scales above 134, where that is no bfloat16, 2^127 and then f2.
+template <int LO> __device__ __forceinline__ uint32_t expand2(uint32_t w, uint32_t f, uint32_t f2, bool large) {
+    const uint32_t b = __byte_perm(w, 0, LO ? 0x3424 : 0x1404);
+    const uint32_t v = mul_bf16x2((b & 0x80008000u) | (b >> 4 & 0x07f007f0u), f);
+    return large ? mul_bf16x2(v, f2) : v;
+}
+
+__global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_constant__ WeightGrad P) {
+    using namespace tc;
+    extern __shared__ __align__(1024) unsigned char dyn[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wq = warp & 3;
+    const uint32_t base = smem_u32(smem), bars = base + OFF_BAR;
+    volatile int &s_abort = *reinterpret_cast<volatile int *>(smem + OFF_BAR + 112);
+    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem + OFF_BAR + 120);
+    const uint32_t tF = bars, tE = tF + 16, pF = tE + 16, pE = pF + 16, cF = pE + 16, cE = cF + 16;       // G and X planes filled, empty; accumulators
+    const int units = P.g_tiles * P.x_groups, unit = blockIdx.x % units, slice = blockIdx.x / units;
+    const int g0 = unit / P.x_groups * WG_G, x0 = unit % P.x_groups * P.x_cols;
+    const int xw = min(P.x_cols, P.m - x0), halves = xw > ACC_COLS ? 2 : 1;
+    const int64_t rb0 = P.row_blocks * slice / P.slices, rb1 = P.row_blocks * (slice + 1) / P.slices;
+
+    if (tid == 0) {
+        s_abort = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(tF + 8 * i, 4); mbar_init(tE + 8 * i, halves);
+            mbar_init(pF + 8 * i, 4); mbar_init(pE + 8 * i, halves);
+            mbar_init(cF + 8 * i, 1); mbar_init(cE + 8 * i, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(smem_u32(&s_tmem), TMEM_COLS);
     pdl_wait();
     pdl_next();
-    __shared__ float sx[WG_ROWS][WG_TILE + 4], sg[WG_ROWS][WG_TILE + 4];
-    const int m0 = blockIdx.x * WG_TILE, c0 = blockIdx.y * WG_TILE, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t r0 = (int64_t)blockIdx.z * chunk, r1 = min(r0 + chunk, n);
-    float acc[4][4] = {}, sum = 0.f;
-    for (int64_t r = r0; r < r1; r += WG_ROWS) {
-        for (int i = threadIdx.x; i < WG_ROWS * WG_TILE; i += 256) {
-            const int k = i / WG_TILE, j = i % WG_TILE;
-            const bool live = r + k < r1;
-            float x = 0.f;
-            if (live && m0 + j < m)
-                x = values2(codes[(r + k) * (int64_t)blocks * 32 + m0 + j]).x * scale_of(scales[(int64_t)((m0 + j) >> 5) * pitch + r + k]);
-            sx[k][j] = x;
-            sg[k][j] = live && c0 + j < cols ? grad[(r + k) * ld + c0 + j] : 0.f;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+
+    if (warp < 4) {
+        regs_dec<REG_ISSUE>();
+        if (warp < halves) {
+            // ---------------- MMAs: a warp per accumulator ----------------
+            const uint32_t idesc = idesc_bf16((min(ACC_COLS, xw - warp * ACC_COLS) + 15) & ~15, true);
+            uint32_t i = 0;
+            bool ok = true;
+            for (int64_t rb = rb0; ok && rb < rb1; rb++, i++) {
+                const uint32_t st = i & 1, ph = (i >> 1) & 1;
+                if (!(ok = warp_wait2(tF + 8 * st, ph, pF + 8 * st, ph, &s_abort))) break;
+                if (!(ok = warp_wait(cE + 8 * warp, (i & 1) ^ 1, &s_abort))) break;
+                fence_after();
+                if (elect_one()) {
+                    const uint32_t a = tmem + 2 * ACC_COLS + st * G_COLS, b = desc_lo(base + OFF_P + st * PLANE + warp * (PLANE / 2), 8192);
+#pragma unroll
+                    for (int q = 2; q >= 0; q--)                       // small parts first
+#pragma unroll
+                        for (int k = 0; k < 4; k++) mma_ts(tmem + warp * ACC_COLS, a + q * 32 + k * 8, b + k * 128, desc_hi(1024), idesc, q < 2 || k > 0);
+                    commit(tE + 8 * st);
+                    commit(pE + 8 * st);
+                    commit(cF + 8 * warp);
+                }
+                __syncwarp();
+            }
+            if (!ok && elect_one()) {                                  // MMAs in flight end before tensor memory is given back
+                commit(cF + 8 * warp);
+                volatile int none = 0;
+                for (int j = 0; j < 2; j++) mbar_wait(cF + 8 * warp, j, &none);
+            }
+            __syncwarp();
         }
-        __syncthreads();
-        for (int k = 0; k < WG_ROWS; k++) {
-            float a[4], b[4];
+    } else if (warp < 8) {
+        regs_dec<REG_G>();
+        // ---------------- G: a thread has a column ----------------
+        const int col = g0 + wq * 32 + lane;
+        const bool live = col < P.cols;
+        const uint32_t raw = base + (wq * 32 + lane) * 4, dst0 = tmem + 2 * ACC_COLS + ((uint32_t)wq << 21);
+        const float *src = P.grad + (live ? col : 0);
+        const auto fetch = [&](int64_t rb, int slot) {
+            if (rb < rb1) {
+                const int64_t r0 = rb * WG_ROWS;
+                const float *p = src + r0 * P.ld;
+                const uint32_t to = raw + slot * RAW_G;
+                const int rows = live ? (int)min((int64_t)WG_ROWS, P.n - r0) : 0;
+                if (rows == WG_ROWS) {
+#pragma unroll 16
+                    for (int k = 0; k < WG_ROWS; k++) { copy4(to + k * 512, p, 4); p += P.ld; }
+                } else {
+                    for (int k = 0; k < WG_ROWS; k++) copy4(to + k * 512, k < rows ? p + k * P.ld : P.grad, k < rows ? 4 : 0);
+                }
+            }
+            copies_end();
+        };
+        float csum = 0.f;
+        fetch(rb0, 0);
+        fetch(rb0 + 1, 1);
+        uint32_t i = 0;
+        int slot = 0;
+        for (int64_t rb = rb0; rb < rb1; rb++, i++) {
+            const uint32_t st = i & 1;
+            fetch(rb + 2, slot == 0 ? 2 : slot - 1);
+            copies_wait<2>();
+            if (!warp_wait(tE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
+            fence_after();
+            const uint32_t from = raw + slot * RAW_G, dst = dst0 + st * G_COLS;
+            f2 bsum = 0;
+#pragma unroll 1
+            for (int k0 = 0; k0 < WG_ROWS; k0 += 16) {
+                uint32_t p[3][8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) { a[i] = sx[k][ty * 4 + i]; b[i] = sg[k][tx * 4 + i]; }
+                for (int k = 0; k < 16; k += 2) {
+                    const f2 v = f2_pack(lds_f1(from + (k0 + k) * 512), lds_f1(from + (k0 + k + 1) * 512));
+                    bsum = f2_add(bsum, v);
+                    split3(v, p[0][k >> 1], p[1][k >> 1], p[2][k >> 1]);
+                }
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += a[i] * b[j];
+                for (int q = 0; q < 3; q++) tmem_st8(dst + q * 32 + (k0 >> 1), p[q]);
+            }
+            const float2 b2 = f2_get(bsum);
+            csum += b2.x + b2.y;
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tF + 8 * st);
+            if (++slot == RAW_STAGES) slot = 0;
         }
-        if (threadIdx.x < WG_TILE)
-            for (int k = 0; k < WG_ROWS; k++) sum += sg[k][threadIdx.x];
-        __syncthreads();
+        copies_wait<0>();
+        if (P.col_part && x0 == 0 && live) P.col_part[(int64_t)slice * P.cols + col] = csum;
+    } else if (warp < 12) {
+        regs_dec<REG_X>();
+        // ---------------- X: a thread has 16 columns of eight rows ----------------
+        const int t = tid - 256, piece = t & 15, row8 = (t >> 4) * 8, col = x0 + piece * 16;
+        const bool live = piece * 16 < P.x_cols && col < P.code_pitch;
+        const uint32_t raw = base + OFF_X + row8 * WG_X + piece * 16, raw_s = base + OFF_S + t * 8;
+        // place of the first stored half piece: eight neighbouring lanes write eight different 16-byte chunks of a row
+        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row8 * 128;
+        const uint8_t *src = P.codes + (live ? col : 0), *src_s = P.scales + (int64_t)(live ? col >> 5 : 0) * P.pitch;
+        const auto fetch = [&](int64_t rb, int slot) {
+            if (live && rb < rb1) {
+                const int64_t r0 = rb * WG_ROWS + row8;
+                const bool any = r0 < P.n;
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    copy16(raw + slot * RAW_X + k * WG_X, r0 + k < P.n ? src + (r0 + k) * P.code_pitch : P.codes, r0 + k < P.n ? 16 : 0);
+                copy8(raw_s + slot * RAW_S, any ? src_s + r0 : P.scales, any ? 8 : 0);      // the pitch is a multiple of 16
+            }
+            copies_end();
+        };
+        fetch(rb0, 0);
+        fetch(rb0 + 1, 1);
+        uint32_t i = 0;
+        int slot = 0;
+        for (int64_t rb = rb0; rb < rb1; rb++, i++) {
+            const uint32_t st = i & 1;
+            fetch(rb + 2, slot == 0 ? 2 : slot - 1);
+            copies_wait<2>();
+            if (!warp_wait(pE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
+            if (live) {
+                uint2 sc;
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(sc.x), "=r"(sc.y) : "r"(raw_s + slot * RAW_S));
+                const int rows = (int)min((int64_t)8, P.n - (rb * WG_ROWS + row8));       // behind the last row scales are not read
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    uint32_t w[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(raw + slot * RAW_X + k * WG_X));
+                    const uint32_t s = k < rows ? ((k < 4 ? sc.x : sc.y) >> (8 * (k & 3))) & 255 : 127;
+                    const bool large = s > 134 && s != 255;
+                    const uint32_t one = s == 255 ? 0x7fc0u : large ? 254u << 7 : (s + 120) << 7, two = large ? (s - 7) << 7 : 0;
+                    const uint32_t f = one | one << 16, f2nd = two | two << 16;
+                    uint32_t a[4], b[4];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        a[2 * j] = expand2<0>(w[j], f, f2nd, large); a[2 * j + 1] = expand2<1>(w[j], f, f2nd, large);
+                        b[2 * j] = expand2<0>(w[2 + j], f, f2nd, large); b[2 * j + 1] = expand2<1>(w[2 + j], f, f2nd, large);
+                    }
+                    const uint32_t to = put + st * PLANE + k * 128, chunk = (piece & 3) * 2;
+                    sts_u4(to + ((chunk + swap) ^ k) * 16, swap ? b : a);
+                    sts_u4(to + ((chunk + 1 - swap) ^ k) * 16, swap ? a : b);
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pF + 8 * st);
+            if (++slot == RAW_STAGES) slot = 0;
+        }
+        copies_wait<0>();
+    } else {
+        regs_inc<REG_ACC>();
+        // ---------------- accumulators: a thread has a column of G, 128 columns of X ----------------
+        const int h = warp >= 16;
+        if (h < halves) {
+            const int wh = min(ACC_COLS, xw - h * ACC_COLS), wm = (wh + 15) & ~15;
+            const uint32_t from = tmem + h * ACC_COLS + ((uint32_t)wq << 21);
+            f2 acc[ACC_COLS / 2];
+#pragma unroll
+            for (int i = 0; i < ACC_COLS / 2; i++) acc[i] = 0;
+            uint32_t cp = 0;
+            for (int64_t rb = rb0; rb < rb1; rb++) {
+                if (!warp_wait(cF + 8 * h, cp, &s_abort)) break;
+                cp ^= 1;
+                fence_after();
+#pragma unroll
+                for (int c = 0; c < ACC_COLS / 8; c++)
+                    if (c * 8 < wm) {
+                        uint32_t v[8];
+                        tmem_ld8(from + c * 8, v);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[c * 4 + i] = f2_add(acc[c * 4 + i], f2_pack(v[2 * i], v[2 * i + 1]));
+                    }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(cE + 8 * h);
+            }
+            const int col = g0 + wq * 32 + lane;
+            if (col < P.cols) {
+                float *to = P.part + ((int64_t)slice * P.m + x0 + h * ACC_COLS) * P.cols + col;
+#pragma unroll
+                for (int i = 0; i < ACC_COLS / 2; i++) {
+                    const float2 v = f2_get(acc[i]);
+                    if (2 * i < wh) to[(int64_t)(2 * i) * P.cols] = v.x;
+                    if (2 * i + 1 < wh) to[(int64_t)(2 * i + 1) * P.cols] = v.y;
+                }
+            }
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int mm = m0 + ty * 4 + i, cc = c0 + tx * 4 + j;
-            if (mm < m && cc < cols) part[((int64_t)blockIdx.z * m + mm) * cols + cc] = acc[i][j];
-        }
-    if (blockIdx.x == 0 && threadIdx.x < WG_TILE && c0 + threadIdx.x < cols) col_part[(int64_t)blockIdx.z * cols + c0 + threadIdx.x] = sum;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 0) tmem_dealloc(tmem, TMEM_COLS);
+    if (tid == 0 && s_abort) atomicOr(P.status, 2);
 }
 
 __global__ void __launch_bounds__(256) weight_finish_kernel(const float *__restrict__ part, const float *__restrict__ col_part, int slices, int64_t size, int cols,
@@ -253,12 +481,35 @@ int check(const char *who, int64_t n, int cols) {
     return AGPT_OK;
 }
 
-int weight_slices(int64_t n, int m, int cols) {
-    const int64_t tiles = (int64_t)((m + WG_TILE - 1) / WG_TILE) * ((cols + WG_TILE - 1) / WG_TILE);
-    int64_t s = (int64_t)vec::sm_count() * 4 / tiles;
-    const int64_t most = (n + WG_ROWS - 1) / WG_ROWS;
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s);
+// One block per (128 columns of the gradient, up to 256 kept columns, slice of the rows): as many slices as fill the SMs, none without rows.
+struct Tiles { int x_groups, x_cols, g_tiles, slices; int64_t row_blocks; };
+Tiles tiles_of(int64_t n, int m, int cols) {
+    Tiles t;
+    t.x_groups = (m + WG_X - 1) / WG_X;
+    t.x_cols = ((m + t.x_groups - 1) / t.x_groups + 31) / 32 * 32;          // split evenly
+    t.x_groups = (m + t.x_cols - 1) / t.x_cols;
+    t.g_tiles = (cols + WG_G - 1) / WG_G;
+    t.row_blocks = (n + WG_ROWS - 1) / WG_ROWS;
+    const int64_t fill = vec::sm_count() / ((int64_t)t.x_groups * t.g_tiles);
+    t.slices = (int)(fill < t.row_blocks ? fill : t.row_blocks);
+    if (t.slices < 1) t.slices = 1;
+    return t;
+}
+int64_t weight_workspace(const Tiles &t, int m, int cols) { return t.slices > 1 ? (int64_t)t.slices * ((int64_t)m * cols + cols) * 4 : 0; }
+
+// once per device: shared memory of the kernel, and the word a wait that ran out is told to
+int weight_setup(int **status) {
+    static std::atomic<int *> word[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && (*status = word[dev].load())) return AGPT_OK;
+    cudaError_t e = cudaFuncSetAttribute(weight_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WG_SMEM);
+    if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "act8_weight_grad: %s", cudaGetErrorString(e));
+    const int *w = nullptr;
+    if (int rc = agpt_step_gemm_status_word(&w)) return rc;
+    *status = const_cast<int *>(w);
+    if (dev >= 0 && dev < 64) word[dev].store(*status);
+    return AGPT_OK;
 }
 
 }  // namespace
@@ -316,7 +567,7 @@ extern "C" int agpt_b200_act8_relu_backward(const float *d_grad, int64_t ld, con
 extern "C" int64_t agpt_b200_act8_weight_grad_workspace_bytes(int64_t n, int m, int cols) {
     if (int rc = check("act8_weight_grad_workspace_bytes", n, m)) return rc;
     if (int rc = check("act8_weight_grad_workspace_bytes", n, cols)) return rc;
-    return (int64_t)weight_slices(n, m, cols) * ((int64_t)m * cols + cols) * 4;
+    return weight_workspace(tiles_of(n, m, cols), m, cols);
 }
 
 extern "C" int agpt_b200_act8_weight_grad(const uint8_t *d_codes, const uint8_t *d_scales, const float *d_grad, int64_t ld, int64_t n, int m, int cols, float *d_weight_grad,
@@ -325,15 +576,24 @@ extern "C" int agpt_b200_act8_weight_grad(const uint8_t *d_codes, const uint8_t 
     if (int rc = check("act8_weight_grad", n, cols)) return rc;
     if (!d_weight_grad || ld < cols || (n && (!d_codes || !d_scales || !d_grad || !vec::aligned(d_codes, 16) || !vec::aligned(d_scales, 16))))
         return agpt_set_error(AGPT_E_ARG, "act8_weight_grad: null or unaligned argument, or bad stride");
-    if (!d_workspace || workspace_bytes < agpt_b200_act8_weight_grad_workspace_bytes(n, m, cols) || !vec::aligned(d_workspace, 16))
+    const Tiles t = tiles_of(n, m, cols);
+    const int64_t size = (int64_t)m * cols, need = weight_workspace(t, m, cols);
+    if (need && (!d_workspace || workspace_bytes < need || !vec::aligned(d_workspace, 16)))
         return agpt_set_error(AGPT_E_ARG, "act8_weight_grad: workspace too small (agpt_b200_act8_weight_grad_workspace_bytes)");
+    const int64_t blocks = (int64_t)t.x_groups * t.g_tiles * t.slices;
+    if (blocks > INT32_MAX || size > (int64_t)INT32_MAX * 128) return agpt_set_error(AGPT_E_LIMIT, "act8_weight_grad: the weight is too large");
     cudaStream_t st = (cudaStream_t)stream;
-    const int slices = weight_slices(n, m, cols);
-    const int64_t chunk = ((n + slices - 1) / slices + WG_ROWS - 1) / WG_ROWS * WG_ROWS, size = (int64_t)m * cols;
-    float *part = (float *)d_workspace, *col_part = part + slices * size;
+    WeightGrad P{};
+    if (int rc = weight_setup(&P.status)) return rc;
     const Shape s = shape_of(n, m);
-    pdl_launch(weight_kernel, dim3((m + WG_TILE - 1) / WG_TILE, (cols + WG_TILE - 1) / WG_TILE, slices), 256, 0, st, d_codes, d_scales, s.pitch, s.blocks, d_grad, ld, n, m, cols,
-               chunk, part, col_part);
-    pdl_launch(weight_finish_kernel, (unsigned)((size + cols + 255) / 256), 256, 0, st, (const float *)part, (const float *)col_part, slices, size, cols, d_weight_grad, d_bias_grad);
+    P.codes = d_codes; P.scales = d_scales; P.grad = d_grad;
+    P.part = t.slices > 1 ? (float *)d_workspace : d_weight_grad;
+    P.col_part = t.slices > 1 ? P.part + t.slices * size : d_bias_grad;
+    P.ld = ld; P.n = n; P.row_blocks = t.row_blocks; P.pitch = s.pitch;
+    P.m = m; P.cols = cols; P.code_pitch = s.blocks * 32; P.slices = t.slices; P.x_cols = t.x_cols; P.x_groups = t.x_groups; P.g_tiles = t.g_tiles;
+    pdl_launch(weight_kernel, (unsigned)blocks, WG_THREADS, WG_SMEM, st, P);
+    if (t.slices > 1)
+        pdl_launch(weight_finish_kernel, (unsigned)((size + cols + 255) / 256), 256, 0, st, (const float *)P.part, (const float *)P.col_part, t.slices, size, cols, d_weight_grad,
+                   d_bias_grad);
     return launch_status("act8_weight_grad");
 }

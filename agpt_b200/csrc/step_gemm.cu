@@ -104,18 +104,6 @@ int allow_smem(Kern k, bool *done) {
 // bit 1: a bounded wait of one of the kernels below ran out
 __device__ int g_step_status = 0;
 
-// a wait of a whole warp whose lanes go on together (tensor-memory instructions follow)
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-}
-
-// two barriers asked for at once (the latencies of two polls overlap)
-__device__ __forceinline__ bool warp_wait2(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, volatile int *abort_flag) {
-    const bool d0 = mbar_try(b0, p0), d1 = mbar_try(b1, p1);
-    if (__all_sync(0xffffffffu, d0 && d1)) return true;
-    return warp_wait(b0, p0, abort_flag) && warp_wait(b1, p1, abort_flag);
-}
-
 // the six partial products, small ones first
 __device__ __forceinline__ void six_products(uint32_t d, uint32_t a, uint32_t b, uint32_t b_plane16, uint32_t b_step16, uint32_t idesc) {
     constexpr int PA[6] = {1, 0, 2, 0, 1, 0}, PB[6] = {1, 2, 0, 1, 0, 0};

@@ -38,6 +38,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// a wait of a whole warp whose lanes go on together (tensor-memory instructions follow)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+// two barriers asked for at once (the latencies of two polls overlap)
+__device__ __forceinline__ bool warp_wait2(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, volatile int *abort_flag) {
+    const bool d0 = mbar_try(b0, p0), d1 = mbar_try(b1, p1);
+    if (__all_sync(0xffffffffu, d0 && d1)) return true;
+    return warp_wait(b0, p0, abort_flag) && warp_wait(b1, p1, abort_flag);
+}
+
 // Between the blocks of a cluster: a shared-memory address of this block as another one has it, barriers there, and plain accesses
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     uint32_t r;
