@@ -756,75 +756,104 @@ def embedding_grad(grad, ids32, vocab, out=None, accumulate=False, serial=False)
 
 
 # rows of float32 or bfloat16, on any device and stream ------------------------------------------------------------------
-def _row_type(t, name, width=None, rows=None):
-    """KV_F32 or KV_BF16 of a 2-D CUDA tensor whose rows are contiguous (a column range of a wider matrix will do)."""
-    import torch
-    if not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.shape[0] and t.stride(1) != 1):
-        raise AgptError(f"{name} must be a 2-D CUDA tensor with contiguous rows")
-    if t.dtype not in (torch.float32, torch.bfloat16):
+# These calls check everything they hand to the library, on tensors that may be tiny: what they ask torch for is looked up once.
+class _Runtime:
+    def __init__(self):
+        import torch
+        self.torch = torch
+        self.kinds = {torch.float32: KV_F32, torch.bfloat16: KV_BF16}
+        self.ids = {torch.int32: 0, torch.int64: 1}
+        self.current_device, self.stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        self.sizes = {}
+
+
+_runtime = None
+
+
+def _rt():
+    global _runtime
+    if _runtime is None:
+        _runtime = _Runtime()
+    return _runtime
+
+
+def _rows(rt, t, name):
+    """(type, rows, columns, elements between rows, device) of a 2-D CUDA tensor with contiguous rows (a column range of a wider matrix will do)."""
+    dev = t.get_device()
+    kind = rt.kinds.get(t.dtype)
+    if dev < 0 or t.dim() != 2:
+        raise AgptError(f"{name} must be a 2-D CUDA tensor")
+    if kind is None:
         raise AgptError(f"{name} has dtype {t.dtype}, expected float32 or bfloat16")
-    if (width is not None and t.shape[1] != width) or (rows is not None and t.shape[0] != rows):
-        raise AgptError(f"{name} has shape {tuple(t.shape)}, expected {(rows if rows is not None else t.shape[0], width if width is not None else t.shape[1])}")
-    return KV_BF16 if t.dtype == torch.bfloat16 else KV_F32
+    n, cols = t.shape
+    ld, inner = t.stride()
+    if n < 2:
+        ld = cols
+    if (inner != 1 and cols > 1 and n) or ld < cols:
+        raise AgptError(f"{name} must have contiguous rows that do not overlap (its strides are {ld} and {inner})")
+    return kind, n, cols, ld, dev
 
 
-def _row_stride(t, name):
-    """Elements from a row to the next; rows that share memory (an expanded tensor) are refused for outputs by the library, for inputs here."""
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        raise AgptError(f"{name} has overlapping rows (stride {ld}): make it contiguous")
+def _rows_like(rt, t, name, kind, n, cols, dev, whole=False):
+    """Elements between rows of a tensor of a known shape, type (None: any of the two) and device.  whole: contiguous."""
+    k, rows, c, ld, d = _rows(rt, t, name)
+    if rows != n or c != cols or d != dev or (kind is not None and k != kind) or (whole and ld != cols):
+        raise AgptError(f"{name} must be a{' contiguous' if whole else ''} tensor {('float32', 'bfloat16')[kind] if kind is not None else ''} of shape {(n, cols)} on cuda:{dev}, "
+                        f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
     return ld
 
 
-def _same_device(ref, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise AgptError(f"{name} is on {t.device}, expected {ref.device}")
-
-
-def _flat(t, name, dtype, numel, ref):
-    if t.dtype != dtype or t.device != ref.device or not t.is_contiguous() or t.numel() != numel:
-        raise AgptError(f"{name} must be a contiguous {dtype} tensor of {numel} elements on {ref.device}")
+def _flat(t, name, dtype, numel, dev):
+    """Address of a contiguous tensor of a known type, size and device; None stays None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() != numel or not t.is_contiguous():
+        raise AgptError(f"{name} must be a contiguous {dtype} tensor of {numel} elements on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _call(ref, what, fn, *args):
-    """fn(*args, stream) on the device of ref and its current stream."""
-    import torch
-    stream = torch.cuda.current_stream(ref.device).cuda_stream
-    if ref.device.index == torch.cuda.current_device():
-        return check(fn(*args, stream), what)
-    with torch.cuda.device(ref.device):
-        return check(fn(*args, stream), what)
+def _on(rt, dev, what, fn, *args):
+    """fn(*args, stream) with the device current and on its current stream."""
+    if rt.current_device() == dev:
+        rc = fn(*args, rt.stream(dev))
+    else:
+        with rt.torch.cuda.device(dev):
+            rc = fn(*args, rt.stream(dev))
+    if rc < 0:
+        check(rc, what)
 
 
-def _scratch_of(ref, what, fn, *args):
-    """Workspace of a call: fresh memory of the caching allocator, so that streams and captured graphs never share it."""
-    import torch
-    with torch.cuda.device(ref.device):
-        need = check(fn(*args), what)
-        return torch.empty(max(int(need), 16), dtype=torch.uint8, device=ref.device), int(need)
+def _scratch_for(rt, t, dev, what, fn, *args):
+    """(tensor or None, bytes): workspace of a call, fresh memory of the caching allocator, so that streams and captured graphs never share it."""
+    need = rt.sizes.get((what, dev, args))
+    if need is None:
+        with rt.torch.cuda.device(dev):
+            need = check(int(fn(*args)), what)
+        if len(rt.sizes) > 4096:
+            rt.sizes.clear()
+        rt.sizes[what, dev, args] = need
+    return (t.new_empty(need, dtype=rt.torch.uint8) if need else None), need
 
 
-def _ids(ids, n, ref):
-    import torch
-    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 1 or not ids.is_contiguous() or ids.device != ref.device or (n is not None and ids.numel() != n):
-        raise AgptError(f"ids must be a contiguous 1-D int32 or int64 tensor{'' if n is None else f' of {n} entries'} on {ref.device}")
-    return int(ids.dtype == torch.int64)
+def _ids(rt, ids, n, dev):
+    wide = rt.ids.get(ids.dtype)
+    if wide is None or ids.dim() != 1 or ids.get_device() != dev or (n is not None and ids.numel() != n) or not ids.is_contiguous():
+        raise AgptError(f"ids must be a contiguous 1-D int32 or int64 tensor{'' if n is None else f' of {n} entries'} on cuda:{dev}")
+    return wide
 
 
 def embedding_lookup(emb, ids, scale: float = 1.0, out=None):
     """out[i] = scale * emb[ids[i]] [n, d_model], of the table's type (float32 or bfloat16); a zero row where an id lies outside the table."""
-    import torch
-    kind = _row_type(emb, "emb")
-    vocab, d = emb.shape
-    wide, ld = _ids(ids, None, emb), _row_stride(emb, "emb")
-    n = ids.numel()
+    rt = _rt()
+    kind, vocab, d, ld, dev = _rows(rt, emb, "emb")
+    if not vocab or not d:
+        raise AgptError("emb has no rows or no columns")
+    wide, n = _ids(rt, ids, None, dev), ids.numel()
     if out is None:
-        out = torch.empty((n, d), dtype=emb.dtype, device=emb.device)
-    elif _row_type(out, "out", d, n) != kind or not out.is_contiguous() or out.device != emb.device:
-        raise AgptError("out must be a contiguous tensor of the table's type on its device")
-    _call(emb, "embedding_lookup", lib().agpt_b200_embedding_lookup, emb.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), n, d, vocab, scale)
+        out = emb.new_empty((n, d))
+    else:
+        _rows_like(rt, out, "out", kind, n, d, dev, whole=True)
+    _on(rt, dev, "embedding_lookup", lib().agpt_b200_embedding_lookup, emb.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), n, d, vocab, scale)
     return out
 
 
@@ -832,38 +861,35 @@ def embedding_grad_sorted(grad, ids, vocab: int, scale: float = 1.0, out=None, a
     """Gradient of embedding_lookup's table, [vocab, d_model]: scale times the sum of grad over the rows of each token, summed in float32 in an
     order that repeats, for vocabularies of any size (embedding_grad keeps tables of up to 400 symbols in shared memory).  out: float32 (the
     default) or bfloat16, added to with accumulate."""
-    import torch
-    kind = _row_type(grad, "grad")
-    n, d = grad.shape
-    wide, ld = _ids(ids, n, grad), _row_stride(grad, "grad")
+    rt = _rt()
+    kind, n, d, ld, dev = _rows(rt, grad, "grad")
+    wide, out_kind = _ids(rt, ids, n, dev), KV_F32
     if out is None:
-        out = (torch.zeros if accumulate else torch.empty)((vocab, d), dtype=torch.float32, device=grad.device)
-    out_kind = _row_type(out, "out", d, vocab)
-    if not out.is_contiguous() or out.device != grad.device:
-        raise AgptError("out must be contiguous and on the device of grad")
+        out = (grad.new_zeros if accumulate else grad.new_empty)((vocab, d), dtype=rt.torch.float32)
+    else:
+        out_kind = rt.kinds.get(out.dtype)
+        _rows_like(rt, out, "out", out_kind, vocab, d, dev, whole=True)
     L = lib()
-    ws, need = _scratch_of(grad, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted_workspace_bytes, n, d, vocab)
-    _call(grad, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted, grad.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), out_kind, n, d, vocab,
-          scale, int(accumulate), ws.data_ptr(), need)
+    ws, need = _scratch_for(rt, grad, dev, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted_workspace_bytes, n, d, vocab)
+    _on(rt, dev, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted, grad.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), out_kind, n, d, vocab, scale,
+        int(accumulate), None if ws is None else ws.data_ptr(), need)
     return out
 
 
-def _rope_args(q, k, pos, cos, sin, q_gain, k_gain):
-    """Sizes and pointers shared by the two directions of qk_norm_rope."""
-    import torch
-    kind = _row_type(q, "q")
-    n, hd = q.shape[0], cos.shape[-1]
-    if _row_type(k, "k", None, n) != kind:
-        raise AgptError("q and k must have the same dtype")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] < 1:
+def _rope_tables(rt, pos, cos, sin, q_gain, k_gain, n, dev):
+    """(head_dim, addresses of gains, positions and tables, positions in the tables)"""
+    f32, shape = rt.torch.float32, cos.shape
+    if len(shape) != 2 or sin.shape != shape or not shape[0]:
         raise AgptError("cos and sin must be [positions, head_dim] tables")
-    if hd < 2 or hd % 2 or hd > 256 or q.shape[1] % hd or k.shape[1] % hd or not q.shape[1] or not k.shape[1]:
-        raise AgptError(f"widths {q.shape[1]} and {k.shape[1]} must be multiples of an even head_dim up to 256, the tables have {hd}")
-    _same_device(q, k=k)
-    tables = [_flat(t, name, torch.float32, t.numel(), q) for name, t in (("cos", cos), ("sin", sin))]
-    at = _flat(pos, "pos", torch.int32, n, q)
-    gains = [None if g is None else _flat(g, name, torch.float32, hd, q) for name, g in (("q_gain", q_gain), ("k_gain", k_gain))]
-    return kind, n, hd, gains + [at] + tables + [cos.shape[0]], [n, q.shape[1] // hd, k.shape[1] // hd, hd]
+    n_pos, hd = shape
+    return hd, (_flat(q_gain, "q_gain", f32, hd, dev), _flat(k_gain, "k_gain", f32, hd, dev), _flat(pos, "pos", rt.torch.int32, n, dev),
+                _flat(cos, "cos", f32, n_pos * hd, dev), _flat(sin, "sin", f32, n_pos * hd, dev), n_pos)
+
+
+def _heads(width, hd, name):
+    if hd < 2 or hd % 2 or hd > 256 or not width or width % hd:
+        raise AgptError(f"{name} has {width} columns: a multiple of the tables' head_dim {hd}, which is even and up to 256, is needed")
+    return width // hd
 
 
 def qk_norm_rope(q, k, q_gain, k_gain, pos, cos, sin, eps: float = 1e-6, k_dtype=None, q_out=None, k_out=None):
@@ -871,38 +897,61 @@ def qk_norm_rope(q, k, q_gain, k_gain, pos, cos, sin, eps: float = 1e-6, k_dtype
     position (as rope_pair_ does), in one pass.  q [n, heads * head_dim], k [n, kv_heads * head_dim], float32 or bfloat16, also as column
     ranges of one matrix; head_dim is the width of the tables.  k_dtype: torch.bfloat16 writes the keys as a bfloat16 store.  Outputs are new
     tensors, or q_out and k_out (q and k themselves will do).  Returns (q, k)."""
-    import torch
-    kind, n, hd, tab, sizes = _rope_args(q, k, pos, cos, sin, q_gain, k_gain)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k_dtype or k.dtype, device=k.device) if k_out is None else k_out
-    types = _row_type(q_out, "q_out", q.shape[1], n), _row_type(k_out, "k_out", k.shape[1], n)
-    if k_dtype is not None and k_out.dtype != k_dtype:
-        raise AgptError(f"k_out has dtype {k_out.dtype}, k_dtype says {k_dtype}")
-    _same_device(q, q_out=q_out, k_out=k_out)
-    _call(q, "qk_norm_rope", lib().agpt_b200_qk_norm_rope, q.data_ptr(), _row_stride(q, "q"), k.data_ptr(), _row_stride(k, "k"), kind, *tab, *sizes, eps,
-          q_out.data_ptr(), _row_stride(q_out, "q_out"), types[0], k_out.data_ptr(), _row_stride(k_out, "k_out"), types[1])
+    rt = _rt()
+    kind, n, qc, q_ld, dev = _rows(rt, q, "q")
+    kc = k.shape[-1]
+    k_ld = _rows_like(rt, k, "k", kind, n, kc, dev)
+    hd, tables = _rope_tables(rt, pos, cos, sin, q_gain, k_gain, n, dev)
+    hq, hk = _heads(qc, hd, "q"), _heads(kc, hd, "k")
+    q_kind = k_kind = kind
+    qo_ld, ko_ld = qc, kc
+    if q_out is None:
+        q_out = q.new_empty((n, qc))
+    else:
+        q_kind = rt.kinds.get(q_out.dtype)
+        qo_ld = _rows_like(rt, q_out, "q_out", q_kind, n, qc, dev)
+    if k_out is None:
+        k_out = k.new_empty((n, kc), dtype=k_dtype)
+        k_kind = rt.kinds.get(k_out.dtype)
+        if k_kind is None:
+            raise AgptError(f"k_dtype {k_dtype}: float32 or bfloat16")
+    else:
+        if k_dtype is not None and k_out.dtype != k_dtype:
+            raise AgptError(f"k_out has dtype {k_out.dtype}, k_dtype says {k_dtype}")
+        k_kind = rt.kinds.get(k_out.dtype)
+        ko_ld = _rows_like(rt, k_out, "k_out", k_kind, n, kc, dev)
+    _on(rt, dev, "qk_norm_rope", lib().agpt_b200_qk_norm_rope, q.data_ptr(), q_ld, k.data_ptr(), k_ld, kind, *tables, n, hq, hk, hd, eps, q_out.data_ptr(), qo_ld, q_kind,
+        k_out.data_ptr(), ko_ld, k_kind)
     return q_out, k_out
 
 
 def qk_norm_rope_backward(dq, dk, q, k, q_gain, k_gain, pos, cos, sin, dq_gain=None, dk_gain=None, eps: float = 1e-6, q_out=None, k_out=None):
     """Gradients of qk_norm_rope with respect to q and k (of their type), from those of its outputs (dq, dk: both float32 or both bfloat16) and
     its inputs.  dq_gain, dk_gain [head_dim] float32 are accumulated into (None: not wanted).  q_out and k_out may be dq and dk."""
-    import torch
-    kind, n, hd, tab, sizes = _rope_args(q, k, pos, cos, sin, q_gain, k_gain)
-    grad_kind = _row_type(dq, "dq", q.shape[1], n)
-    if _row_type(dk, "dk", k.shape[1], n) != grad_kind:
-        raise AgptError("dq and dk must have the same dtype")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
-    if _row_type(q_out, "q_out", q.shape[1], n) != kind or _row_type(k_out, "k_out", k.shape[1], n) != kind:
-        raise AgptError("q_out and k_out must have the dtype of q and k")
-    _same_device(q, dq=dq, dk=dk, q_out=q_out, k_out=k_out)
-    gains = [None if g is None else _flat(g, name, torch.float32, hd, q) for name, g in (("dq_gain", dq_gain), ("dk_gain", dk_gain))]
-    L = lib()
-    ws, need = _scratch_of(q, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward_workspace_bytes, hd)
-    _call(q, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward, dq.data_ptr(), _row_stride(dq, "dq"), dk.data_ptr(), _row_stride(dk, "dk"), grad_kind,
-          q.data_ptr(), _row_stride(q, "q"), k.data_ptr(), _row_stride(k, "k"), kind, *tab, *sizes, eps, q_out.data_ptr(), _row_stride(q_out, "q_out"),
-          k_out.data_ptr(), _row_stride(k_out, "k_out"), *gains, ws.data_ptr(), need)
+    rt = _rt()
+    kind, n, qc, q_ld, dev = _rows(rt, q, "q")
+    kc = k.shape[-1]
+    k_ld = _rows_like(rt, k, "k", kind, n, kc, dev)
+    grad_kind = rt.kinds.get(dq.dtype)
+    dq_ld, dk_ld = _rows_like(rt, dq, "dq", grad_kind, n, qc, dev), _rows_like(rt, dk, "dk", grad_kind, n, kc, dev)
+    hd, tables = _rope_tables(rt, pos, cos, sin, q_gain, k_gain, n, dev)
+    hq, hk = _heads(qc, hd, "q"), _heads(kc, hd, "k")
+    qo_ld, ko_ld = qc, kc
+    if q_out is None:
+        q_out = q.new_empty((n, qc))
+    else:
+        qo_ld = _rows_like(rt, q_out, "q_out", kind, n, qc, dev)
+    if k_out is None:
+        k_out = k.new_empty((n, kc))
+    else:
+        ko_ld = _rows_like(rt, k_out, "k_out", kind, n, kc, dev)
+    f32 = rt.torch.float32
+    gains = _flat(dq_gain, "dq_gain", f32, hd, dev), _flat(dk_gain, "dk_gain", f32, hd, dev)
+    L, ws, need = lib(), None, 0
+    if gains != (None, None):
+        ws, need = _scratch_for(rt, q, dev, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward_workspace_bytes, hd)
+    _on(rt, dev, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward, dq.data_ptr(), dq_ld, dk.data_ptr(), dk_ld, grad_kind, q.data_ptr(), q_ld, k.data_ptr(), k_ld,
+        kind, *tables, n, hq, hk, hd, eps, q_out.data_ptr(), qo_ld, k_out.data_ptr(), ko_ld, *gains, None if ws is None else ws.data_ptr(), need)
     return q_out, k_out
 
 
@@ -913,14 +962,15 @@ class Act8:
     __slots__ = ("codes", "scales", "cols")
 
     def __init__(self, codes, scales, cols: int):
-        import torch
-        n, blocks = codes.shape[0], -(-cols // 32)
-        if cols < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.device != scales.device or not codes.is_contiguous() or \
-                not scales.is_contiguous() or tuple(codes.shape) != (n, blocks * 32) or tuple(scales.shape) != (blocks, (n + 15) // 16 * 16):
+        u8, blocks = _rt().torch.uint8, (cols + 31) // 32
+        n, c = codes.shape if codes.dim() == 2 else (0, 0)
+        if cols < 1 or c != blocks * 32 or codes.dtype is not u8 or scales.dtype is not u8 or scales.shape != (blocks, (n + 15) // 16 * 16) or not codes.is_contiguous() or \
+                not scales.is_contiguous():
             raise AgptError(f"an 8-bit activation of {cols} columns has contiguous uint8 codes [n, {blocks * 32}] and scales [{blocks}, n rounded up to 16]")
-        if not codes.is_cuda or (codes.data_ptr() | scales.data_ptr()) & 15:
-            raise AgptError("codes and scales must be CUDA tensors on 16-byte boundaries")
-        self.codes, self.scales, self.cols = codes, scales, int(cols)
+        dev = codes.get_device()
+        if dev < 0 or scales.get_device() != dev or (codes.data_ptr() | scales.data_ptr()) & 15:
+            raise AgptError("codes and scales must be tensors of one CUDA device on 16-byte boundaries")
+        self.codes, self.scales, self.cols = codes, scales, cols
 
     @property
     def shape(self):
@@ -934,62 +984,63 @@ class Act8:
 def act8_pack(x) -> Act8:
     """x [n, cols] (float32 or bfloat16) as an 8-bit checkpoint: at most 2^-4 of a value is lost, or half a step of the block's smallest code; what is not
     zero does not become zero."""
-    import torch
-    kind = _row_type(x, "x")
-    n, cols = x.shape
-    if cols < 1:
+    rt = _rt()
+    kind, n, cols, ld, dev = _rows(rt, x, "x")
+    if not cols:
         raise AgptError("x has no columns")
-    blocks = -(-cols // 32)
-    a = Act8(torch.empty((n, blocks * 32), dtype=torch.uint8, device=x.device), torch.empty((blocks, (n + 15) // 16 * 16), dtype=torch.uint8, device=x.device), cols)
-    _call(x, "act8_pack", lib().agpt_b200_act8_pack, x.data_ptr(), _row_stride(x, "x"), kind, a.codes.data_ptr(), a.scales.data_ptr(), n, cols)
+    blocks, u8 = (cols + 31) // 32, rt.torch.uint8
+    a = Act8.__new__(Act8)
+    a.codes, a.scales, a.cols = x.new_empty((n, blocks * 32), dtype=u8), x.new_empty((blocks, (n + 15) // 16 * 16), dtype=u8), cols
+    _on(rt, dev, "act8_pack", lib().agpt_b200_act8_pack, x.data_ptr(), ld, kind, a.codes.data_ptr(), a.scales.data_ptr(), n, cols)
     return a
 
 
 def act8_unpack(a: Act8):
     """The values of a checkpoint, float32 [n, cols]."""
-    import torch
-    out = torch.empty(a.shape, dtype=torch.float32, device=a.device)
-    _call(out, "act8_unpack", lib().agpt_b200_act8_unpack, a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr(), *a.shape)
+    rt, n = _rt(), a.codes.shape[0]
+    out = a.codes.new_empty((n, a.cols), dtype=rt.torch.float32)
+    _on(rt, a.codes.get_device(), "act8_unpack", lib().agpt_b200_act8_unpack, a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr(), n, a.cols)
     return out
 
 
-def _act8_grad(a, grad, cols):
-    import torch
-    if _row_type(grad, "grad", cols, a.shape[0]) != KV_F32:
-        raise AgptError("grad must be float32")
-    _same_device(grad, activation=a)
-    return _row_stride(grad, "grad")
+def _act8_grad(rt, a, grad):
+    """(rows, columns, elements between rows, device) of a float32 gradient with the rows of a"""
+    kind, n, cols, ld, dev = _rows(rt, grad, "grad")
+    if kind != KV_F32 or n != a.codes.shape[0] or dev != a.codes.get_device():
+        raise AgptError(f"grad must be float32 with {a.codes.shape[0]} rows on {a.device}, got {grad.dtype} {tuple(grad.shape)} on {grad.device}")
+    return n, cols, ld, dev
 
 
 def act8_relu_backward(grad, a: Act8, out=None):
     """grad where the kept activation is above 0, else 0: relu_backward with the mask read from a checkpoint.  out may be grad."""
-    import torch
-    ld = _act8_grad(a, grad, a.cols)
+    rt = _rt()
+    n, cols, ld, dev = _act8_grad(rt, a, grad)
+    if cols != a.cols:
+        raise AgptError(f"grad has {cols} columns, the activation {a.cols}")
     if out is None:
-        out = torch.empty(grad.shape, dtype=torch.float32, device=grad.device)
-    elif _row_type(out, "out", *grad.shape[::-1]) != KV_F32 or not out.is_contiguous() or out.device != grad.device:
-        raise AgptError("out must be a contiguous float32 tensor of the shape of grad on its device")
-    _call(grad, "act8_relu_backward", lib().agpt_b200_act8_relu_backward, grad.data_ptr(), ld, a.codes.data_ptr(), out.data_ptr(), *a.shape)
+        out = grad.new_empty((n, cols))
+    else:
+        _rows_like(rt, out, "out", KV_F32, n, cols, dev, whole=True)
+    _on(rt, dev, "act8_relu_backward", lib().agpt_b200_act8_relu_backward, grad.data_ptr(), ld, a.codes.data_ptr(), out.data_ptr(), n, cols)
     return out
 
 
 def act8_weight_grad(a: Act8, grad, out=None, bias_grad: bool = True):
     """(X^T grad [cols of a, cols of grad], column sums of grad): weight and bias gradients of a projection whose input was kept in 8 bits, accurate to
     float32 over the kept values.  bias_grad=False: (weight gradient, None)."""
-    import torch
-    n, m = a.shape
-    ld, cols = _act8_grad(a, grad, grad.shape[-1]), grad.shape[1]
-    if cols < 1:
+    rt = _rt()
+    n, cols, ld, dev = _act8_grad(rt, a, grad)
+    if not cols:
         raise AgptError("grad has no columns")
     if out is None:
-        out = torch.empty((m, cols), dtype=torch.float32, device=grad.device)
-    elif _row_type(out, "out", cols, m) != KV_F32 or not out.is_contiguous() or out.device != grad.device:
-        raise AgptError(f"out must be a contiguous float32 tensor of shape {(m, cols)} on the device of grad")
-    db = torch.empty(cols, dtype=torch.float32, device=grad.device) if bias_grad else None
+        out = grad.new_empty((a.cols, cols))
+    else:
+        _rows_like(rt, out, "out", KV_F32, a.cols, cols, dev, whole=True)
+    db = grad.new_empty(cols) if bias_grad else None
     L = lib()
-    ws, need = _scratch_of(grad, "act8_weight_grad", L.agpt_b200_act8_weight_grad_workspace_bytes, n, m, cols)
-    _call(grad, "act8_weight_grad", L.agpt_b200_act8_weight_grad, a.codes.data_ptr(), a.scales.data_ptr(), grad.data_ptr(), ld, n, m, cols, out.data_ptr(),
-          None if db is None else db.data_ptr(), ws.data_ptr(), need)
+    ws, need = _scratch_for(rt, grad, dev, "act8_weight_grad", L.agpt_b200_act8_weight_grad_workspace_bytes, n, a.cols, cols)
+    _on(rt, dev, "act8_weight_grad", L.agpt_b200_act8_weight_grad, a.codes.data_ptr(), a.scales.data_ptr(), grad.data_ptr(), ld, n, a.cols, cols, out.data_ptr(),
+        None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out, db
 
 

@@ -44,7 +44,7 @@ def test_the_library_refuses_before_it_launches():
         L.agpt_b200_act8_unpack(some, None, some, 4, 32, None),
         L.agpt_b200_act8_relu_backward(some, 32, None, some, 4, 32, None),
         L.agpt_b200_act8_weight_grad(some, some, some, 7, 4, 32, 8, some, None, some, 1 << 30, None),
-        L.agpt_b200_act8_weight_grad(some, some, some, 8, 4, 32, 8, some, None, some, 4, None),
+        L.agpt_b200_act8_weight_grad(some, some, some, 8, 100_000, 32, 8, some, None, some, 4, None),                     # workspace too small
         L.agpt_b200_act8_weight_grad(some, some, some, 8, 4, 0, 8, some, None, some, 1 << 30, None),
     ]
     assert bad == [-1] * len(bad)
