@@ -173,36 +173,29 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // ---- weight gradient: dW[m][N] = X^T G, db[N] = column sums of G ----------------------------------------------------------------------
 // On tcgen05, float32-accurate: a kept value is exact in bfloat16, an element of G is the exact sum of three, so a product is three MMAs.  The MMA's rows are
 // 128 columns of G: a converting thread owns one, walks down the rows and writes its packed pairs to tensor memory.  Up to 256 columns of X, n contiguous, come
-// through shared memory, so that a split of G serves all of them.  Loads are asynchronous copies of 4 (G) and 16 bytes (X) into places that only the copying
-// thread reads again: no alignment is asked of G, and no barrier stands between a copy and its use.  An accumulator leaves tensor memory after every 64 rows
-// and is added in registers (tensor cores truncate when they add).  Blocks own (G tile, X columns, slice of the rows); slices are added in order.
+// through shared memory, so that a split of G serves all of them.  TMA brings the raw rows; rows of G that it cannot take (off 16-byte boundaries) are copied four
+// bytes at a time by the threads that convert them.  Blocks own (G tile, X columns, slice of the rows); slices are added in order.
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
-constexpr int WG_THREADS = 640;                        // four warps that issue MMAs, four on G, four on X, two groups of four that own an accumulator
-constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 128 * 8, PLANE = WG_ROWS * WG_X * 2;
-constexpr uint32_t OFF_X = RAW_STAGES * RAW_G, OFF_S = OFF_X + RAW_STAGES * RAW_X, OFF_P = OFF_S + RAW_STAGES * RAW_S, OFF_BAR = OFF_P + 2 * PLANE;
-constexpr size_t WG_SMEM = OFF_BAR + 128 + 1024;
+constexpr int WG_THREADS = 640;                        // four warps that load and issue MMAs, four on G, four on X, two groups of four that own an accumulator
+constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 8 * WG_ROWS, PLANE = WG_ROWS * WG_X * 2;
+constexpr uint32_t OFF_X = RAW_STAGES * RAW_G, OFF_P = OFF_X + RAW_STAGES * RAW_X, OFF_S = OFF_P + 2 * PLANE, OFF_BAR = OFF_S + RAW_STAGES * RAW_S;
+constexpr size_t WG_SMEM = OFF_BAR + 256 + 1024;
 static_assert(WG_SMEM <= 232448 && OFF_P % 1024 == 0, "shared memory");
 constexpr int ACC_COLS = 128, G_COLS = 96, TMEM_COLS = 512;
-constexpr int REG_ISSUE = 40, REG_G = 72, REG_X = 64, REG_ACC = 152;
+constexpr int REG_ISSUE = 40, REG_G = 64, REG_X = 72, REG_ACC = 152;
 static_assert(REG_ISSUE + REG_G + REG_X + 2 * REG_ACC <= 5 * 96, "setmaxnreg draws on the registers of the launch");
 
-struct WeightGrad {
-    const uint8_t *codes, *scales;
+struct alignas(64) WeightGrad {
+    CUtensorMap map_g, map_x, map_s;
     const float *grad;
     float *part, *col_part;            // [slices][m][cols], [slices][cols]: the results themselves if there is one slice
-    int64_t ld, n, row_blocks, pitch;
-    int m, cols, code_pitch, slices, x_cols, x_groups, g_tiles;
+    int64_t ld, n, row_blocks;
+    int m, cols, slices, x_cols, x_groups, g_tiles;
     int *status;
 };
 
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy8(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -211,23 +204,24 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// Two codes (bytes lo, lo + 1 of w) as bfloat16 values times 2^(scale - 127).  Sign, exponent and fraction of a code moved to their places in a bfloat16 make its
-// value times 2^-120, subnormal ones included; f = 2^(scale - 7), and for scales above 134, where that is no bfloat16, 2^127 and then f2.
-template <int LO> __device__ __forceinline__ uint32_t expand2(uint32_t w, uint32_t f, uint32_t f2, bool large) {
-    const uint32_t b = __byte_perm(w, 0, LO ? 0x3424 : 0x1404);
-    const uint32_t v = mul_bf16x2((b & 0x80008000u) | (b >> 4 & 0x07f007f0u), f);
-    return large ? mul_bf16x2(v, f2) : v;
+// Two codes (bytes 0, 1 or 2, 3 of w) as bfloat16 values times 2^(scale - 127).  Sign, exponent and fraction of a code moved to their places in a bfloat16 make its
+// value times 2^-120, subnormal ones included; f = 2^(scale - 7).
+template <int HIGH> __device__ __forceinline__ uint32_t expand2(uint32_t w, uint32_t f) {
+    const uint32_t b = __byte_perm(w, 0, HIGH ? 0x3424 : 0x1404);
+    return mul_bf16x2((b & 0x80008000u) | (b >> 4 & 0x07f007f0u), f);
 }
 
+template <bool TMA_G>
 __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_constant__ WeightGrad P) {
     using namespace tc;
     extern __shared__ __align__(1024) unsigned char dyn[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wq = warp & 3;
     const uint32_t base = smem_u32(smem), bars = base + OFF_BAR;
-    volatile int &s_abort = *reinterpret_cast<volatile int *>(smem + OFF_BAR + 112);
-    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem + OFF_BAR + 120);
-    const uint32_t tF = bars, tE = tF + 16, pF = tE + 16, pE = pF + 16, cF = pE + 16, cE = cF + 16;       // G and X planes filled, empty; accumulators
+    volatile int &s_abort = *reinterpret_cast<volatile int *>(smem + OFF_BAR + 240);
+    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem + OFF_BAR + 248);
+    // G and X planes filled, empty; accumulators; raw rows of G and X filled, empty
+    const uint32_t tF = bars, tE = tF + 16, pF = tE + 16, pE = pF + 16, cF = pE + 16, cE = cF + 16, gF = cE + 16, gE = gF + 24, xF = gE + 24, xE = xF + 24;
     const int units = P.g_tiles * P.x_groups, unit = blockIdx.x % units, slice = blockIdx.x / units;
     const int g0 = unit / P.x_groups * WG_G, x0 = unit % P.x_groups * P.x_cols;
     const int xw = min(P.x_cols, P.m - x0), halves = xw > ACC_COLS ? 2 : 1;
@@ -240,6 +234,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
             mbar_init(pF + 8 * i, 4); mbar_init(pE + 8 * i, halves);
             mbar_init(cF + 8 * i, 1); mbar_init(cE + 8 * i, 4);
         }
+        for (int i = 0; i < RAW_STAGES; i++) { mbar_init(gF + 8 * i, 1); mbar_init(gE + 8 * i, 4); mbar_init(xF + 8 * i, 1); mbar_init(xE + 8 * i, 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), TMEM_COLS);
@@ -252,7 +247,32 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
 
     if (warp < 4) {
         regs_dec<REG_ISSUE>();
-        if (warp < halves) {
+        if (warp == 2 && lane == 0) {
+            // ---------------- loads ----------------
+            int slot = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int64_t rb = rb0; ok && rb < rb1; rb++) {
+                const int y = (int)(rb * WG_ROWS);
+                if (TMA_G) {
+                    if (!(ok = mbar_wait(gE + 8 * slot, ph ^ 1, &s_abort))) break;
+                    mbar_expect(gF + 8 * slot, RAW_G);
+                    tma_load_2d(base + slot * RAW_G, &P.map_g, g0, y, gF + 8 * slot);
+                }
+                if (!(ok = mbar_wait(xE + 8 * slot, ph ^ 1, &s_abort))) break;
+                mbar_expect(xF + 8 * slot, (uint32_t)(WG_ROWS * P.x_cols + RAW_S));
+                tma_load_2d(base + OFF_X + slot * RAW_X, &P.map_x, x0, y, xF + 8 * slot);
+                tma_load_2d(base + OFF_S + slot * RAW_S, &P.map_s, y, x0 >> 5, xF + 8 * slot);
+                if (++slot == RAW_STAGES) { slot = 0; ph ^= 1; }
+            }
+            if (!ok) {                                                 // copies in flight end before the block does
+                volatile int none = 0;
+                for (int i = 0; i < RAW_STAGES; i++) {
+                    if (TMA_G) mbar_wait(gF + 8 * i, ph, &none);
+                    mbar_wait(xF + 8 * i, ph, &none);
+                }
+            }
+        } else if (warp < halves) {
             // ---------------- MMAs: a warp per accumulator ----------------
             const uint32_t idesc = idesc_bf16((min(ACC_COLS, xw - warp * ACC_COLS) + 15) & ~15, true);
             uint32_t i = 0;
@@ -288,31 +308,31 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
         const bool live = col < P.cols;
         const uint32_t raw = base + (wq * 32 + lane) * 4, dst0 = tmem + 2 * ACC_COLS + ((uint32_t)wq << 21);
         const float *src = P.grad + (live ? col : 0);
+        // without TMA a thread copies what it converts, so that nothing but the end of its own copies has to be waited for
         const auto fetch = [&](int64_t rb, int slot) {
             if (rb < rb1) {
                 const int64_t r0 = rb * WG_ROWS;
                 const float *p = src + r0 * P.ld;
                 const uint32_t to = raw + slot * RAW_G;
                 const int rows = live ? (int)min((int64_t)WG_ROWS, P.n - r0) : 0;
-                if (rows == WG_ROWS) {
-#pragma unroll 16
-                    for (int k = 0; k < WG_ROWS; k++) { copy4(to + k * 512, p, 4); p += P.ld; }
-                } else {
-                    for (int k = 0; k < WG_ROWS; k++) copy4(to + k * 512, k < rows ? p + k * P.ld : P.grad, k < rows ? 4 : 0);
-                }
+#pragma unroll 8
+                for (int k = 0; k < WG_ROWS; k++) { copy4(to + k * 512, k < rows ? p : P.grad, k < rows ? 4 : 0); p += P.ld; }
             }
             copies_end();
         };
+        if (!TMA_G) { fetch(rb0, 0); fetch(rb0 + 1, 1); }
         float csum = 0.f;
-        fetch(rb0, 0);
-        fetch(rb0 + 1, 1);
-        uint32_t i = 0;
+        uint32_t i = 0, gp = 0;
         int slot = 0;
         for (int64_t rb = rb0; rb < rb1; rb++, i++) {
             const uint32_t st = i & 1;
-            fetch(rb + 2, slot == 0 ? 2 : slot - 1);
-            copies_wait<2>();
-            if (!warp_wait(tE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
+            if (TMA_G) {
+                if (!warp_wait2(gF + 8 * slot, gp, tE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
+            } else {
+                fetch(rb + 2, slot == 0 ? 2 : slot - 1);
+                copies_wait<2>();
+                if (!warp_wait(tE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
+            }
             fence_after();
             const uint32_t from = raw + slot * RAW_G, dst = dst0 + st * G_COLS;
             f2 bsum = 0;
@@ -333,69 +353,67 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
             tmem_wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(tF + 8 * st);
-            if (++slot == RAW_STAGES) slot = 0;
+            if (lane == 0) { if (TMA_G) mbar_arrive(gE + 8 * slot); mbar_arrive(tF + 8 * st); }
+            if (++slot == RAW_STAGES) { slot = 0; gp ^= 1; }
         }
-        copies_wait<0>();
+        if (!TMA_G) copies_wait<0>();
         if (P.col_part && x0 == 0 && live) P.col_part[(int64_t)slice * P.cols + col] = csum;
     } else if (warp < 12) {
         regs_dec<REG_X>();
         // ---------------- X: a thread has 16 columns of eight rows ----------------
-        const int t = tid - 256, piece = t & 15, row8 = (t >> 4) * 8, col = x0 + piece * 16;
-        const bool live = piece * 16 < P.x_cols && col < P.code_pitch;
-        const uint32_t raw = base + OFF_X + row8 * WG_X + piece * 16, raw_s = base + OFF_S + t * 8;
+        const int t = tid - 256, piece = t & 15, row8 = (t >> 4) * 8;
+        const bool live = piece * 16 < P.x_cols;
+        const uint32_t raw = base + OFF_X + row8 * P.x_cols + piece * 16, raw_s = base + OFF_S + (piece >> 1) * WG_ROWS + row8;
         // place of the first stored half piece: eight neighbouring lanes write eight different 16-byte chunks of a row
-        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row8 * 128;
-        const uint8_t *src = P.codes + (live ? col : 0), *src_s = P.scales + (int64_t)(live ? col >> 5 : 0) * P.pitch;
-        const auto fetch = [&](int64_t rb, int slot) {
-            if (live && rb < rb1) {
-                const int64_t r0 = rb * WG_ROWS + row8;
-                const bool any = r0 < P.n;
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    copy16(raw + slot * RAW_X + k * WG_X, r0 + k < P.n ? src + (r0 + k) * P.code_pitch : P.codes, r0 + k < P.n ? 16 : 0);
-                copy8(raw_s + slot * RAW_S, any ? src_s + r0 : P.scales, any ? 8 : 0);      // the pitch is a multiple of 16
-            }
-            copies_end();
-        };
-        fetch(rb0, 0);
-        fetch(rb0 + 1, 1);
-        uint32_t i = 0;
+        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row8 * 128, chunk = (piece & 3) * 2;
+        uint32_t i = 0, xp = 0;
         int slot = 0;
         for (int64_t rb = rb0; rb < rb1; rb++, i++) {
             const uint32_t st = i & 1;
-            fetch(rb + 2, slot == 0 ? 2 : slot - 1);
-            copies_wait<2>();
-            if (!warp_wait(pE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
+            if (!warp_wait2(xF + 8 * slot, xp, pE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
             if (live) {
-                uint2 sc;
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(sc.x), "=r"(sc.y) : "r"(raw_s + slot * RAW_S));
-                const int rows = (int)min((int64_t)8, P.n - (rb * WG_ROWS + row8));       // behind the last row scales are not read
+                uint32_t sc[2];
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(sc[0]), "=r"(sc[1]) : "r"(raw_s + slot * RAW_S));
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    uint32_t w[4];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(raw + slot * RAW_X + k * WG_X));
-                    const uint32_t s = k < rows ? ((k < 4 ? sc.x : sc.y) >> (8 * (k & 3))) & 255 : 127;
-                    const bool large = s > 134 && s != 255;
-                    const uint32_t one = s == 255 ? 0x7fc0u : large ? 254u << 7 : (s + 120) << 7, two = large ? (s - 7) << 7 : 0;
-                    const uint32_t f = one | one << 16, f2nd = two | two << 16;
-                    uint32_t a[4], b[4];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        a[2 * j] = expand2<0>(w[j], f, f2nd, large); a[2 * j + 1] = expand2<1>(w[j], f, f2nd, large);
-                        b[2 * j] = expand2<0>(w[2 + j], f, f2nd, large); b[2 * j + 1] = expand2<1>(w[2 + j], f, f2nd, large);
+                for (int k0 = 0; k0 < 8; k0 += 4) {
+                    if (rb == P.row_blocks - 1) {                      // scales behind the last row may hold anything
+                        const int64_t rows = P.n - (rb * WG_ROWS + row8 + k0);
+                        const uint32_t past = rows >= 4 ? 0 : rows <= 0 ? 0xffffffffu : 0xffffffffu << (8 * (int)rows);
+                        sc[k0 >> 2] = (sc[k0 >> 2] & ~past) | (0x7f7f7f7fu & past);
                     }
-                    const uint32_t to = put + st * PLANE + k * 128, chunk = (piece & 3) * 2;
-                    sts_u4(to + ((chunk + swap) ^ k) * 16, swap ? b : a);
-                    sts_u4(to + ((chunk + 1 - swap) ^ k) * 16, swap ? a : b);
+                    uint32_t w[4][4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
+                                     : "r"(raw + slot * RAW_X + (k0 + k) * P.x_cols));
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t s = sc[k0 >> 2] >> (8 * k) & 255;
+                        // 2^(scale - 7): no bfloat16 above 134, where 2^127 comes first and the rest second
+                        const bool large = s > 134 && s != 255;
+                        const uint32_t one = s == 255 ? 0x7fc0u : large ? 254u << 7 : (s + 120) << 7, f = one | one << 16;
+                        uint32_t a[4], b[4];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            a[2 * j] = expand2<0>(w[k][j], f); a[2 * j + 1] = expand2<1>(w[k][j], f);
+                            b[2 * j] = expand2<0>(w[k][2 + j], f); b[2 * j + 1] = expand2<1>(w[k][2 + j], f);
+                        }
+                        if (__any_sync(__activemask(), large)) {
+                            const uint32_t two = large ? (s - 7) << 7 : 0x3f80u, f2nd = two | two << 16;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) { a[j] = mul_bf16x2(a[j], f2nd); b[j] = mul_bf16x2(b[j], f2nd); }
+                        }
+                        const uint32_t to = put + st * PLANE + (k0 + k) * 128;
+                        sts_u4(to + ((chunk + swap) ^ (k0 + k)) * 16, swap ? b : a);
+                        sts_u4(to + ((chunk + 1 - swap) ^ (k0 + k)) * 16, swap ? a : b);
+                    }
                 }
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(pF + 8 * st);
-            if (++slot == RAW_STAGES) slot = 0;
+            if (lane == 0) { mbar_arrive(xE + 8 * slot); mbar_arrive(pF + 8 * st); }
+            if (++slot == RAW_STAGES) { slot = 0; xp ^= 1; }
         }
-        copies_wait<0>();
     } else {
         regs_inc<REG_ACC>();
         // ---------------- accumulators: a thread has a column of G, 128 columns of X ----------------
@@ -412,12 +430,12 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
                 cp ^= 1;
                 fence_after();
 #pragma unroll
-                for (int c = 0; c < ACC_COLS / 8; c++)
-                    if (c * 8 < wm) {
-                        uint32_t v[8];
-                        tmem_ld8(from + c * 8, v);
+                for (int c = 0; c < ACC_COLS / 16; c++)
+                    if (c * 16 < wm) {
+                        uint32_t v[16];
+                        tmem_ld16(from + c * 16, v);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[c * 4 + i] = f2_add(acc[c * 4 + i], f2_pack(v[2 * i], v[2 * i + 1]));
+                        for (int i = 0; i < 8; i++) acc[c * 8 + i] = f2_add(acc[c * 8 + i], f2_pack(v[2 * i], v[2 * i + 1]));
                     }
                 fence_before();
                 __syncwarp();
@@ -497,18 +515,40 @@ Tiles tiles_of(int64_t n, int m, int cols) {
 }
 int64_t weight_workspace(const Tiles &t, int m, int cols) { return t.slices > 1 ? (int64_t)t.slices * ((int64_t)m * cols + cols) * 4 : 0; }
 
-// once per device: shared memory of the kernel, and the word a wait that ran out is told to
+// once per device: shared memory of the kernels, and the word a wait that ran out is told to
 int weight_setup(int **status) {
     static std::atomic<int *> word[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && (*status = word[dev].load())) return AGPT_OK;
-    cudaError_t e = cudaFuncSetAttribute(weight_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WG_SMEM);
+    cudaError_t e = cudaFuncSetAttribute(weight_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WG_SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(weight_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WG_SMEM);
     if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "act8_weight_grad: %s", cudaGetErrorString(e));
     const int *w = nullptr;
     if (int rc = agpt_step_gemm_status_word(&w)) return rc;
     *status = const_cast<int *>(w);
     if (dev >= 0 && dev < 64) word[dev].store(*status);
+    return AGPT_OK;
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// rows x cols of `type`, boxes of box_rows x box_cols without swizzle; what lies outside reads as zero
+int encode_map(CUtensorMap *m, CUtensorMapDataType type, const void *p, int64_t rows, int64_t cols, int64_t ld_bytes, int box_rows, int box_cols) {
+    static std::atomic<EncodeFn> found{nullptr};
+    EncodeFn fn = found.load();
+    if (!fn) {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q);
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !f) return agpt_set_error(AGPT_E_CUDA, "cuTensorMapEncodeTiled not found");
+        found.store(fn = (EncodeFn)f);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, es[2] = {1, 1};
+    const CUresult r = fn(m, type, 2, const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return agpt_set_error(AGPT_E_CUDA, "tensor map of %lld x %lld: error %d", (long long)rows, (long long)cols, (int)r);
     return AGPT_OK;
 }
 
@@ -581,17 +621,26 @@ extern "C" int agpt_b200_act8_weight_grad(const uint8_t *d_codes, const uint8_t 
     if (need && (!d_workspace || workspace_bytes < need || !vec::aligned(d_workspace, 16)))
         return agpt_set_error(AGPT_E_ARG, "act8_weight_grad: workspace too small (agpt_b200_act8_weight_grad_workspace_bytes)");
     const int64_t blocks = (int64_t)t.x_groups * t.g_tiles * t.slices;
-    if (blocks > INT32_MAX || size > (int64_t)INT32_MAX * 128) return agpt_set_error(AGPT_E_LIMIT, "act8_weight_grad: the weight is too large");
+    if (n > (int64_t)INT32_MAX - WG_ROWS || blocks > INT32_MAX || size > (int64_t)INT32_MAX * 128) return agpt_set_error(AGPT_E_LIMIT, "act8_weight_grad: more than 2^31 rows, or the weight is too large");
     cudaStream_t st = (cudaStream_t)stream;
     WeightGrad P{};
     if (int rc = weight_setup(&P.status)) return rc;
     const Shape s = shape_of(n, m);
-    P.codes = d_codes; P.scales = d_scales; P.grad = d_grad;
+    P.grad = d_grad;
     P.part = t.slices > 1 ? (float *)d_workspace : d_weight_grad;
     P.col_part = t.slices > 1 ? P.part + t.slices * size : d_bias_grad;
-    P.ld = ld; P.n = n; P.row_blocks = t.row_blocks; P.pitch = s.pitch;
-    P.m = m; P.cols = cols; P.code_pitch = s.blocks * 32; P.slices = t.slices; P.x_cols = t.x_cols; P.x_groups = t.x_groups; P.g_tiles = t.g_tiles;
-    pdl_launch(weight_kernel, (unsigned)blocks, WG_THREADS, WG_SMEM, st, P);
+    P.ld = ld; P.n = n; P.row_blocks = t.row_blocks;
+    P.m = m; P.cols = cols; P.slices = t.slices; P.x_cols = t.x_cols; P.x_groups = t.x_groups; P.g_tiles = t.g_tiles;
+    // a row stride is a multiple of 16 bytes and below 2^40; one row has none
+    const bool tma = ld % 4 == 0 && vec::aligned(d_grad, 16) && ld < (int64_t)1 << 36;
+    if (n) {
+        if (int rc = encode_map(&P.map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, d_codes, n, s.blocks * 32, s.blocks * 32, WG_ROWS, t.x_cols)) return rc;
+        if (int rc = encode_map(&P.map_s, CU_TENSOR_MAP_DATA_TYPE_UINT8, d_scales, s.blocks, s.pitch, s.pitch, 8, WG_ROWS)) return rc;
+        if (tma)
+            if (int rc = encode_map(&P.map_g, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, d_grad, n, cols, ld * 4, WG_ROWS, WG_G)) return rc;
+    }
+    if (tma) pdl_launch(weight_kernel<true>, (unsigned)blocks, WG_THREADS, WG_SMEM, st, P);
+    else pdl_launch(weight_kernel<false>, (unsigned)blocks, WG_THREADS, WG_SMEM, st, P);
     if (t.slices > 1)
         pdl_launch(weight_finish_kernel, (unsigned)((size + cols + 255) / 256), 256, 0, st, (const float *)P.part, (const float *)P.col_part, t.slices, size, cols, d_weight_grad,
                    d_bias_grad);
