@@ -278,26 +278,26 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
             uint32_t i = 0;
             bool ok = true;
             for (int64_t rb = rb0; ok && rb < rb1; rb++, i++) {
-                const uint32_t st = i & 1, ph = (i >> 1) & 1;
+                const uint32_t st = i & 1, ph = (i >> 1) & 1, turn = i >> 1, own = halves == 2 ? warp : turn & 1, uses = halves == 2 ? turn : turn >> 1;
+                if (st == 0 && !(ok = warp_wait(cE + 8 * own, (uses & 1) ^ 1, &s_abort))) break;
                 if (!(ok = warp_wait2(tF + 8 * st, ph, pF + 8 * st, ph, &s_abort))) break;
-                if (!(ok = warp_wait(cE + 8 * warp, (i & 1) ^ 1, &s_abort))) break;
                 fence_after();
                 if (elect_one()) {
                     const uint32_t a = tmem + 2 * ACC_COLS + st * G_COLS, b = desc_lo(base + OFF_P + st * PLANE + warp * (PLANE / 2), 8192);
 #pragma unroll
                     for (int q = 2; q >= 0; q--)                       // small parts first
 #pragma unroll
-                        for (int k = 0; k < 4; k++) mma_ts(tmem + warp * ACC_COLS, a + q * 32 + k * 8, b + k * 128, desc_hi(1024), idesc, q < 2 || k > 0);
+                        for (int k = 0; k < 4; k++) mma_ts(tmem + own * ACC_COLS, a + q * 32 + k * 8, b + k * 128, desc_hi(1024), idesc, st || q < 2 || k > 0);
                     commit(tE + 8 * st);
                     commit(pE + 8 * st);
-                    commit(cF + 8 * warp);
+                    if (st || rb + 1 == rb1) commit(cF + 8 * own);
                 }
                 __syncwarp();
             }
             if (!ok && elect_one()) {                                  // MMAs in flight end before tensor memory is given back
-                commit(cF + 8 * warp);
+                commit(tE);
                 volatile int none = 0;
-                for (int j = 0; j < 2; j++) mbar_wait(cF + 8 * warp, j, &none);
+                for (int j = 0; j < 2; j++) mbar_wait(tE, j, &none);
             }
             __syncwarp();
         }
@@ -374,39 +374,49 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
             if (live) {
                 uint32_t sc[2];
                 asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(sc[0]), "=r"(sc[1]) : "r"(raw_s + slot * RAW_S));
+                if (rb == P.row_blocks - 1)                            // scales behind the last row may hold anything
 #pragma unroll
-                for (int k0 = 0; k0 < 8; k0 += 4) {
-                    if (rb == P.row_blocks - 1) {                      // scales behind the last row may hold anything
-                        const int64_t rows = P.n - (rb * WG_ROWS + row8 + k0);
+                    for (int k = 0; k < 2; k++) {
+                        const int64_t rows = P.n - (rb * WG_ROWS + row8 + 4 * k);
                         const uint32_t past = rows >= 4 ? 0 : rows <= 0 ? 0xffffffffu : 0xffffffffu << (8 * (int)rows);
-                        sc[k0 >> 2] = (sc[k0 >> 2] & ~past) | (0x7f7f7f7fu & past);
+                        sc[k] = (sc[k] & ~past) | (0x7f7f7f7fu & past);
                     }
-                    uint32_t w[4][4];
+                // 2^(scale - 7) is a bfloat16 up to 134; above, 2^127 and a second factor (255: NaN)
+                const bool large = __vcmpgtu4(sc[0], 0x86868686u) | __vcmpgtu4(sc[1], 0x86868686u);
+                uint32_t from = raw + slot * RAW_X, to = put + st * PLANE;
+#pragma unroll 1
+                for (uint32_t k = 0; k < 8; k += 2) {
+                    uint32_t w[2][4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
-                                     : "r"(raw + slot * RAW_X + (k0 + k) * P.x_cols));
+                    for (int j = 0; j < 2; j++) {
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][0]), "=r"(w[j][1]) : "r"(from + j * P.x_cols + swap * 8));
+                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2]), "=r"(w[j][3]) : "r"(from + j * P.x_cols + 8 - swap * 8));
+                    }
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t s = sc[k0 >> 2] >> (8 * k) & 255;
-                        // 2^(scale - 7): no bfloat16 above 134, where 2^127 comes first and the rest second
-                        const bool large = s > 134 && s != 255;
-                        const uint32_t one = s == 255 ? 0x7fc0u : large ? 254u << 7 : (s + 120) << 7, f = one | one << 16;
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t s = (k < 4 ? sc[0] : sc[1]) >> (8 * ((k & 2) + j)) & 255;
                         uint32_t a[4], b[4];
+                        if (!large) {
+                            const uint32_t f = (s + 120) * 0x00800080u;
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            a[2 * j] = expand2<0>(w[k][j], f); a[2 * j + 1] = expand2<1>(w[k][j], f);
-                            b[2 * j] = expand2<0>(w[k][2 + j], f); b[2 * j + 1] = expand2<1>(w[k][2 + j], f);
-                        }
-                        if (__any_sync(__activemask(), large)) {
-                            const uint32_t two = large ? (s - 7) << 7 : 0x3f80u, f2nd = two | two << 16;
+                            for (int i = 0; i < 2; i++) {
+                                a[2 * i] = expand2<0>(w[j][i], f); a[2 * i + 1] = expand2<1>(w[j][i], f);
+                                b[2 * i] = expand2<0>(w[j][2 + i], f); b[2 * i + 1] = expand2<1>(w[j][2 + i], f);
+                            }
+                        } else {
+                            const uint32_t one = s > 134 ? 254u * 0x00800080u : (s + 120) * 0x00800080u;
+                            const uint32_t two = s == 255 ? 0x7fc07fc0u : s > 134 ? (s - 7) * 0x00800080u : 0x3f803f80u;
 #pragma unroll
-                            for (int j = 0; j < 4; j++) { a[j] = mul_bf16x2(a[j], f2nd); b[j] = mul_bf16x2(b[j], f2nd); }
+                            for (int i = 0; i < 2; i++) {
+                                a[2 * i] = mul_bf16x2(expand2<0>(w[j][i], one), two); a[2 * i + 1] = mul_bf16x2(expand2<1>(w[j][i], one), two);
+                                b[2 * i] = mul_bf16x2(expand2<0>(w[j][2 + i], one), two); b[2 * i + 1] = mul_bf16x2(expand2<1>(w[j][2 + i], one), two);
+                            }
                         }
-                        const uint32_t to = put + st * PLANE + (k0 + k) * 128;
-                        sts_u4(to + ((chunk + swap) ^ (k0 + k)) * 16, swap ? b : a);
-                        sts_u4(to + ((chunk + 1 - swap) ^ (k0 + k)) * 16, swap ? a : b);
+                        sts_u4(to + j * 128 + ((chunk + swap) ^ (k + j)) * 16, a);
+                        sts_u4(to + j * 128 + ((chunk + 1 - swap) ^ (k + j)) * 16, b);
                     }
+                    from += 2 * P.x_cols;
+                    to += 256;
                 }
             }
             fence_async_smem();
@@ -417,39 +427,51 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
     } else {
         regs_inc<REG_ACC>();
         // ---------------- accumulators: a thread has a column of G, 128 columns of X ----------------
-        const int h = warp >= 16;
-        if (h < halves) {
-            const int wh = min(ACC_COLS, xw - h * ACC_COLS), wm = (wh + 15) & ~15;
-            const uint32_t from = tmem + h * ACC_COLS + ((uint32_t)wq << 21);
-            f2 acc[ACC_COLS / 2];
+        const int group = warp >= 16, h = halves == 2 ? group : 0;
+        const int wh = min(ACC_COLS, xw - h * ACC_COLS), wm = (wh + 15) & ~15;
+        const uint32_t from = tmem + group * ACC_COLS + ((uint32_t)wq << 21);
+        f2 acc[ACC_COLS / 2];
 #pragma unroll
-            for (int i = 0; i < ACC_COLS / 2; i++) acc[i] = 0;
-            uint32_t cp = 0;
-            for (int64_t rb = rb0; rb < rb1; rb++) {
-                if (!warp_wait(cF + 8 * h, cp, &s_abort)) break;
-                cp ^= 1;
-                fence_after();
+        for (int i = 0; i < ACC_COLS / 2; i++) acc[i] = 0;
+        uint32_t cp = 0;
+        for (int64_t turn = halves == 2 ? 0 : group; turn < (rb1 - rb0 + 1) >> 1; turn += halves == 2 ? 1 : 2) {
+            if (!warp_wait(cF + 8 * group, cp, &s_abort)) break;
+            cp ^= 1;
+            fence_after();
 #pragma unroll
-                for (int c = 0; c < ACC_COLS / 16; c++)
-                    if (c * 16 < wm) {
-                        uint32_t v[16];
-                        tmem_ld16(from + c * 16, v);
+            for (int c = 0; c < ACC_COLS / 16; c++)
+                if (c * 16 < wm) {
+                    uint32_t v[16];
+                    tmem_ld16(from + c * 16, v);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) acc[c * 8 + i] = f2_add(acc[c * 8 + i], f2_pack(v[2 * i], v[2 * i + 1]));
-                    }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(cE + 8 * h);
-            }
-            const int col = g0 + wq * 32 + lane;
-            if (col < P.cols) {
-                float *to = P.part + ((int64_t)slice * P.m + x0 + h * ACC_COLS) * P.cols + col;
+                    for (int i = 0; i < 8; i++) acc[c * 8 + i] = f2_add(acc[c * 8 + i], f2_pack(v[2 * i], v[2 * i + 1]));
+                }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(cE + 8 * group);
+        }
+        const int own = wq * 32 + lane;
+        if (halves == 1) {                                             // both groups have sums of the same columns
+            float *meet = reinterpret_cast<float *>(smem + OFF_P) + own;
+            asm volatile("bar.sync 1, 256;" ::: "memory");             // both have seen their last MMAs end: nothing reads the planes any more
+            if (group)
 #pragma unroll
                 for (int i = 0; i < ACC_COLS / 2; i++) {
                     const float2 v = f2_get(acc[i]);
-                    if (2 * i < wh) to[(int64_t)(2 * i) * P.cols] = v.x;
-                    if (2 * i + 1 < wh) to[(int64_t)(2 * i + 1) * P.cols] = v.y;
+                    meet[2 * i * 128] = v.x; meet[(2 * i + 1) * 128] = v.y;
                 }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (!group)
+#pragma unroll
+                for (int i = 0; i < ACC_COLS / 2; i++) acc[i] = f2_add(acc[i], f2_pack(meet[2 * i * 128], meet[(2 * i + 1) * 128]));
+        }
+        if (g0 + own < P.cols && group < halves) {
+            float *to = P.part + ((int64_t)slice * P.m + x0 + h * ACC_COLS) * P.cols + g0 + own;
+#pragma unroll
+            for (int i = 0; i < ACC_COLS / 2; i++) {
+                const float2 v = f2_get(acc[i]);
+                if (2 * i < wh) to[(int64_t)(2 * i) * P.cols] = v.x;
+                if (2 * i + 1 < wh) to[(int64_t)(2 * i + 1) * P.cols] = v.y;
             }
         }
     }
