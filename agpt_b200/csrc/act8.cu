@@ -176,14 +176,14 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // through shared memory, so that a split of G serves all of them.  TMA brings the raw rows; rows of G that it cannot take (off 16-byte boundaries) are copied four
 // bytes at a time by the threads that convert them.  Blocks own (G tile, X columns, slice of the rows); slices are added in order.
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
-constexpr int WG_THREADS = 640;                        // four warps that load and issue MMAs, four on G, four on X, two groups of four that own an accumulator
+constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, two groups of four that own an accumulator
 constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 8 * WG_ROWS, PLANE = WG_ROWS * WG_X * 2;
 constexpr uint32_t OFF_X = RAW_STAGES * RAW_G, OFF_P = OFF_X + RAW_STAGES * RAW_X, OFF_S = OFF_P + 2 * PLANE, OFF_BAR = OFF_S + RAW_STAGES * RAW_S;
 constexpr size_t WG_SMEM = OFF_BAR + 256 + 1024;
 static_assert(WG_SMEM <= 232448 && OFF_P % 1024 == 0, "shared memory");
 constexpr int ACC_COLS = 128, G_COLS = 96, TMEM_COLS = 512;
-constexpr int REG_ISSUE = 40, REG_G = 64, REG_X = 72, REG_ACC = 152;
-static_assert(REG_ISSUE + REG_G + REG_X + 2 * REG_ACC <= 5 * 96, "setmaxnreg draws on the registers of the launch");
+constexpr int REG_ISSUE = 32, REG_G = 64, REG_X = 40, REG_ACC = 152;
+static_assert(REG_ISSUE + REG_G + 2 * REG_X + 2 * REG_ACC <= 6 * 80, "setmaxnreg draws on the registers of the launch");
 
 struct alignas(64) WeightGrad {
     CUtensorMap map_g, map_x, map_s;
@@ -207,8 +207,9 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // Two codes (bytes 0, 1 or 2, 3 of w) as bfloat16 values times 2^(scale - 127).  Sign, exponent and fraction of a code moved to their places in a bfloat16 make its
 // value times 2^-120, subnormal ones included; f = 2^(scale - 7).
 template <int HIGH> __device__ __forceinline__ uint32_t expand2(uint32_t w, uint32_t f) {
-    const uint32_t b = __byte_perm(w, 0, HIGH ? 0x3424 : 0x1404);
-    return mul_bf16x2((b & 0x80008000u) | (b >> 4 & 0x07f007f0u), f);
+    uint32_t b;                                                        // each code behind eight copies of its sign
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(b) : "r"(w), "n"(HIGH ? 0xb3a2 : 0x9180));
+    return mul_bf16x2(b << 4 & 0x87f087f0u, f);
 }
 
 template <bool TMA_G>
@@ -231,10 +232,10 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
         s_abort = 0;
         for (int i = 0; i < 2; i++) {
             mbar_init(tF + 8 * i, 4); mbar_init(tE + 8 * i, halves);
-            mbar_init(pF + 8 * i, 4); mbar_init(pE + 8 * i, halves);
+            mbar_init(pF + 8 * i, 8); mbar_init(pE + 8 * i, halves);
             mbar_init(cF + 8 * i, 1); mbar_init(cE + 8 * i, 4);
         }
-        for (int i = 0; i < RAW_STAGES; i++) { mbar_init(gF + 8 * i, 1); mbar_init(gE + 8 * i, 4); mbar_init(xF + 8 * i, 1); mbar_init(xE + 8 * i, 4); }
+        for (int i = 0; i < RAW_STAGES; i++) { mbar_init(gF + 8 * i, 1); mbar_init(gE + 8 * i, 4); mbar_init(xF + 8 * i, 1); mbar_init(xE + 8 * i, 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), TMEM_COLS);
@@ -358,65 +359,49 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
         }
         if (!TMA_G) copies_wait<0>();
         if (P.col_part && x0 == 0 && live) P.col_part[(int64_t)slice * P.cols + col] = csum;
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         regs_dec<REG_X>();
-        // ---------------- X: a thread has 16 columns of eight rows ----------------
-        const int t = tid - 256, piece = t & 15, row8 = (t >> 4) * 8;
+        // ---------------- X: a thread has 16 columns of four rows ----------------
+        const int t = tid - 256, piece = t & 15, row4 = (t >> 4) * 4;
         const bool live = piece * 16 < P.x_cols;
-        const uint32_t raw = base + OFF_X + row8 * P.x_cols + piece * 16, raw_s = base + OFF_S + (piece >> 1) * WG_ROWS + row8;
+        const uint32_t raw = base + OFF_X + row4 * P.x_cols + piece * 16, raw_s = base + OFF_S + (piece >> 1) * WG_ROWS + row4;
         // place of the first stored half piece: eight neighbouring lanes write eight different 16-byte chunks of a row
-        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row8 * 128, chunk = (piece & 3) * 2;
+        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row4 * 128;
+        const uint32_t even = row4 & 4, at = (piece & 3) * 2 + swap, at2 = at ^ 1;
         uint32_t i = 0, xp = 0;
         int slot = 0;
         for (int64_t rb = rb0; rb < rb1; rb++, i++) {
             const uint32_t st = i & 1;
             if (!warp_wait2(xF + 8 * slot, xp, pE + 8 * st, ((i >> 1) & 1) ^ 1, &s_abort)) break;
             if (live) {
-                uint32_t sc[2];
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(sc[0]), "=r"(sc[1]) : "r"(raw_s + slot * RAW_S));
-                if (rb == P.row_blocks - 1)                            // scales behind the last row may hold anything
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int64_t rows = P.n - (rb * WG_ROWS + row8 + 4 * k);
-                        const uint32_t past = rows >= 4 ? 0 : rows <= 0 ? 0xffffffffu : 0xffffffffu << (8 * (int)rows);
-                        sc[k] = (sc[k] & ~past) | (0x7f7f7f7fu & past);
-                    }
+                uint32_t sc;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc) : "r"(raw_s + slot * RAW_S));
+                if (rb == P.row_blocks - 1) {                          // scales behind the last row may hold anything
+                    const int64_t rows = P.n - (rb * WG_ROWS + row4);
+                    const uint32_t past = rows >= 4 ? 0 : rows <= 0 ? 0xffffffffu : 0xffffffffu << (8 * (int)rows);
+                    sc = (sc & ~past) | (0x7f7f7f7fu & past);
+                }
                 // 2^(scale - 7) is a bfloat16 up to 134; above, 2^127 and a second factor (255: NaN)
-                const bool large = __vcmpgtu4(sc[0], 0x86868686u) | __vcmpgtu4(sc[1], 0x86868686u);
-                uint32_t from = raw + slot * RAW_X, to = put + st * PLANE;
-#pragma unroll 1
-                for (uint32_t k = 0; k < 8; k += 2) {
-                    uint32_t w[2][4];
+                const bool large = __vcmpgtu4(sc, 0x86868686u);
+                const uint32_t from = raw + slot * RAW_X, to = put + st * PLANE;
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][0]), "=r"(w[j][1]) : "r"(from + j * P.x_cols + swap * 8));
-                        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][2]), "=r"(w[j][3]) : "r"(from + j * P.x_cols + 8 - swap * 8));
+                for (uint32_t k = 0; k < 4; k++) {
+                    uint32_t w[4], a[4], b[4];
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from + k * P.x_cols + swap * 8));
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "r"(from + k * P.x_cols + 8 - swap * 8));
+                    const uint32_t s = sc >> (8 * k) & 255, f = (s > 134 ? 254u : s + 120) * 0x00800080u;
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        a[2 * i] = expand2<0>(w[i], f); a[2 * i + 1] = expand2<1>(w[i], f);
+                        b[2 * i] = expand2<0>(w[2 + i], f); b[2 * i + 1] = expand2<1>(w[2 + i], f);
                     }
+                    if (large) {
+                        const uint32_t two = s == 255 ? 0x7fc07fc0u : s > 134 ? (s - 7) * 0x00800080u : 0x3f803f80u;
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t s = (k < 4 ? sc[0] : sc[1]) >> (8 * ((k & 2) + j)) & 255;
-                        uint32_t a[4], b[4];
-                        if (!large) {
-                            const uint32_t f = (s + 120) * 0x00800080u;
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                a[2 * i] = expand2<0>(w[j][i], f); a[2 * i + 1] = expand2<1>(w[j][i], f);
-                                b[2 * i] = expand2<0>(w[j][2 + i], f); b[2 * i + 1] = expand2<1>(w[j][2 + i], f);
-                            }
-                        } else {
-                            const uint32_t one = s > 134 ? 254u * 0x00800080u : (s + 120) * 0x00800080u;
-                            const uint32_t two = s == 255 ? 0x7fc07fc0u : s > 134 ? (s - 7) * 0x00800080u : 0x3f803f80u;
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                a[2 * i] = mul_bf16x2(expand2<0>(w[j][i], one), two); a[2 * i + 1] = mul_bf16x2(expand2<1>(w[j][i], one), two);
-                                b[2 * i] = mul_bf16x2(expand2<0>(w[j][2 + i], one), two); b[2 * i + 1] = mul_bf16x2(expand2<1>(w[j][2 + i], one), two);
-                            }
-                        }
-                        sts_u4(to + j * 128 + ((chunk + swap) ^ (k + j)) * 16, a);
-                        sts_u4(to + j * 128 + ((chunk + 1 - swap) ^ (k + j)) * 16, b);
+                        for (int i = 0; i < 4; i++) { a[i] = mul_bf16x2(a[i], two); b[i] = mul_bf16x2(b[i], two); }
                     }
-                    from += 2 * P.x_cols;
-                    to += 256;
+                    sts_u4(to + k * 128 + (at ^ (even | k)) * 16, a);
+                    sts_u4(to + k * 128 + (at2 ^ (even | k)) * 16, b);
                 }
             }
             fence_async_smem();
@@ -427,7 +412,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
     } else {
         regs_inc<REG_ACC>();
         // ---------------- accumulators: a thread has a column of G, 128 columns of X ----------------
-        const int group = warp >= 16, h = halves == 2 ? group : 0;
+        const int group = warp >= 20, h = halves == 2 ? group : 0;
         const int wh = min(ACC_COLS, xw - h * ACC_COLS), wm = (wh + 15) & ~15;
         const uint32_t from = tmem + group * ACC_COLS + ((uint32_t)wq << 21);
         f2 acc[ACC_COLS / 2];
