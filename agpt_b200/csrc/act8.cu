@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // through shared memory, so that a split of G serves all of them.  TMA brings the raw rows; rows of G that it cannot take (off 16-byte boundaries) are copied four
 // bytes at a time by the threads that convert them.  Blocks own (G tile, X columns, slice of the rows); slices are added in order.
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
-constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, two groups of four that own an accumulator
+constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, eight on the accumulators
 constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 8 * WG_ROWS, PLANE = WG_ROWS * WG_X * 2;
 constexpr uint32_t OFF_X = RAW_STAGES * RAW_G, OFF_P = OFF_X + RAW_STAGES * RAW_X, OFF_S = OFF_P + 2 * PLANE, OFF_BAR = OFF_S + RAW_STAGES * RAW_S;
 constexpr size_t WG_SMEM = OFF_BAR + 256 + 1024;
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
         for (int i = 0; i < 2; i++) {
             mbar_init(tF + 8 * i, 4); mbar_init(tE + 8 * i, halves);
             mbar_init(pF + 8 * i, 8); mbar_init(pE + 8 * i, halves);
-            mbar_init(cF + 8 * i, 1); mbar_init(cE + 8 * i, 4);
+            mbar_init(cF + 8 * i, 1); mbar_init(cE + 8 * i, 8);
         }
         for (int i = 0; i < RAW_STAGES; i++) { mbar_init(gF + 8 * i, 1); mbar_init(gE + 8 * i, 4); mbar_init(xF + 8 * i, 1); mbar_init(xE + 8 * i, 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -411,54 +411,53 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
         }
     } else {
         regs_inc<REG_ACC>();
-        // ---------------- accumulators: a thread has a column of G, 128 columns of X ----------------
-        const int group = warp >= 20, h = halves == 2 ? group : 0;
-        const int wh = min(ACC_COLS, xw - h * ACC_COLS), wm = (wh + 15) & ~15;
-        const uint32_t from = tmem + group * ACC_COLS + ((uint32_t)wq << 21);
-        f2 acc[ACC_COLS / 2];
+        // ---------------- accumulators: a thread has a column of G, 64 columns of X of each accumulator ----------------
+        // Both groups drain each accumulator, half of its columns each, so that it is soon free for the next MMAs.
+        const int group = warp >= 20, own = wq * 32 + lane;
+        const uint32_t from = tmem + group * (ACC_COLS / 2) + ((uint32_t)wq << 21);
+        f2 acc[2][ACC_COLS / 4];
 #pragma unroll
-        for (int i = 0; i < ACC_COLS / 2; i++) acc[i] = 0;
-        uint32_t cp = 0;
-        for (int64_t turn = halves == 2 ? 0 : group; turn < (rb1 - rb0 + 1) >> 1; turn += halves == 2 ? 1 : 2) {
-            if (!warp_wait(cF + 8 * group, cp, &s_abort)) break;
-            cp ^= 1;
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < ACC_COLS / 4; i++) acc[h][i] = 0;
+        uint32_t cp[2] = {0, 0};
+        const auto drain = [&](int a, f2 (&sum)[ACC_COLS / 4], int columns) {
+            if (!warp_wait(cF + 8 * a, cp[a], &s_abort)) return false;
+            cp[a] ^= 1;
             fence_after();
 #pragma unroll
-            for (int c = 0; c < ACC_COLS / 16; c++)
-                if (c * 16 < wm) {
+            for (int c = 0; c < ACC_COLS / 2; c += 16)
+                if (c + group * (ACC_COLS / 2) < columns) {
                     uint32_t v[16];
-                    tmem_ld16(from + c * 16, v);
+                    tmem_ld16(from + a * ACC_COLS + c, v);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) acc[c * 8 + i] = f2_add(acc[c * 8 + i], f2_pack(v[2 * i], v[2 * i + 1]));
+                    for (int i = 0; i < 8; i++) sum[c / 2 + i] = f2_add(sum[c / 2 + i], f2_pack(v[2 * i], v[2 * i + 1]));
                 }
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(cE + 8 * group);
+            if (lane == 0) mbar_arrive(cE + 8 * a);
+            return true;
+        };
+        const int64_t turns = (rb1 - rb0 + 1) >> 1;
+        if (halves == 2) {
+            for (int64_t t = 0; t < turns; t++)
+                if (!drain(0, acc[0], ACC_COLS) || !drain(1, acc[1], xw - ACC_COLS)) break;
+        } else {
+            for (int64_t t = 0; t < turns; t += 2)
+                if (!drain(0, acc[0], xw) || (t + 1 < turns && !drain(1, acc[0], xw))) break;
         }
-        const int own = wq * 32 + lane;
-        if (halves == 1) {                                             // both groups have sums of the same columns
-            float *meet = reinterpret_cast<float *>(smem + OFF_P) + own;
-            asm volatile("bar.sync 1, 256;" ::: "memory");             // both have seen their last MMAs end: nothing reads the planes any more
-            if (group)
+        if (g0 + own < P.cols)
 #pragma unroll
-                for (int i = 0; i < ACC_COLS / 2; i++) {
-                    const float2 v = f2_get(acc[i]);
-                    meet[2 * i * 128] = v.x; meet[(2 * i + 1) * 128] = v.y;
+            for (int h = 0; h < 2; h++) {
+                const int first = h * ACC_COLS + group * (ACC_COLS / 2);
+                float *to = P.part + ((int64_t)slice * P.m + x0 + first) * P.cols + g0 + own;
+#pragma unroll
+                for (int i = 0; i < ACC_COLS / 4; i++) {
+                    const float2 v = f2_get(acc[h][i]);
+                    if (first + 2 * i < xw) to[(int64_t)(2 * i) * P.cols] = v.x;
+                    if (first + 2 * i + 1 < xw) to[(int64_t)(2 * i + 1) * P.cols] = v.y;
                 }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (!group)
-#pragma unroll
-                for (int i = 0; i < ACC_COLS / 2; i++) acc[i] = f2_add(acc[i], f2_pack(meet[2 * i * 128], meet[(2 * i + 1) * 128]));
-        }
-        if (g0 + own < P.cols && group < halves) {
-            float *to = P.part + ((int64_t)slice * P.m + x0 + h * ACC_COLS) * P.cols + g0 + own;
-#pragma unroll
-            for (int i = 0; i < ACC_COLS / 2; i++) {
-                const float2 v = f2_get(acc[i]);
-                if (2 * i < wh) to[(int64_t)(2 * i) * P.cols] = v.x;
-                if (2 * i + 1 < wh) to[(int64_t)(2 * i + 1) * P.cols] = v.y;
             }
-        }
     }
     fence_before();
     __syncthreads();
