@@ -466,22 +466,51 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
     if (tid == 0 && s_abort) atomicOr(P.status, 2);
 }
 
+// Sums of the slices in order.  A warp has 128 numbers; of many slices, the eight warps of a block have the same numbers and a run of the slices each.  The numbers are
+// the weight gradient's and, behind it, the bias gradient's.
+constexpr int SPLIT_FROM = 16;
+template <bool SPLIT>
 __global__ void __launch_bounds__(256) weight_finish_kernel(const float *__restrict__ part, const float *__restrict__ col_part, int slices, int64_t size, int cols,
-                                                             float *__restrict__ dw, float *__restrict__ db) {
+                                                             float *__restrict__ dw, float *__restrict__ db, int64_t weight_blocks) {
     pdl_wait();
     pdl_next();
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < size) {
-        float t = 0.f;
+    __shared__ float s[8][128];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const bool bias = blockIdx.x >= weight_blocks;
+    const int64_t first = (blockIdx.x - (bias ? weight_blocks : 0)) * (SPLIT ? 128 : 1024) + (SPLIT ? 0 : w * 128), total = bias ? cols : size;
+    const float *from = bias ? col_part : part;
+    const int s0 = SPLIT ? slices * w / 8 : 0, s1 = SPLIT ? slices * (w + 1) / 8 : slices;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    if ((total & 3) == 0) {                                            // rows of slices on 16-byte boundaries
+        if (first + lane * 4 < total)
 #pragma unroll 8
-        for (int s = 0; s < slices; s++) t += __ldcs(part + s * size + i);
-        dw[i] = t;
-    } else if (db && i < size + cols) {
-        const int c = (int)(i - size);
-        float t = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < slices; s++) t += __ldcs(col_part + (int64_t)s * cols + c);
-        db[c] = t;
+            for (int k = s0; k < s1; k++) {
+                const float4 v = __ldcs(reinterpret_cast<const float4 *>(from + k * total + first) + lane);
+                t[0] += v.x; t[1] += v.y; t[2] += v.z; t[3] += v.w;
+            }
+    } else {
+#pragma unroll 2
+        for (int k = s0; k < s1; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (first + lane * 4 + i < total) t[i] += __ldcs(from + k * total + first + lane * 4 + i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[w][lane * 4 + i] = t[i];
+    if (!SPLIT) {
+        __syncwarp();
+#pragma unroll
+        for (int i = lane; i < 128; i += 32)
+            if (first + i < total) (bias ? db : dw)[first + i] = s[w][i];
+        return;
+    }
+    __syncthreads();
+    const int64_t i = first + threadIdx.x;
+    if (threadIdx.x < 128 && i < total) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum += s[k][threadIdx.x];
+        (bias ? db : dw)[i] = sum;
     }
 }
 
@@ -519,7 +548,7 @@ Tiles tiles_of(int64_t n, int m, int cols) {
     if (t.slices < 1) t.slices = 1;
     return t;
 }
-int64_t weight_workspace(const Tiles &t, int m, int cols) { return t.slices > 1 ? (int64_t)t.slices * ((int64_t)m * cols + cols) * 4 : 0; }
+int64_t weight_workspace(const Tiles &t, int m, int cols) { return t.slices > 1 ? ((int64_t)t.slices * m * cols + 3) / 4 * 16 + (int64_t)t.slices * cols * 4 : 0; }
 
 // once per device: shared memory of the kernels, and the word a wait that ran out is told to
 int weight_setup(int **status) {
@@ -634,7 +663,7 @@ extern "C" int agpt_b200_act8_weight_grad(const uint8_t *d_codes, const uint8_t 
     const Shape s = shape_of(n, m);
     P.grad = d_grad;
     P.part = t.slices > 1 ? (float *)d_workspace : d_weight_grad;
-    P.col_part = t.slices > 1 ? P.part + t.slices * size : d_bias_grad;
+    P.col_part = t.slices > 1 ? P.part + (t.slices * size + 3) / 4 * 4 : d_bias_grad;
     P.ld = ld; P.n = n; P.row_blocks = t.row_blocks;
     P.m = m; P.cols = cols; P.slices = t.slices; P.x_cols = t.x_cols; P.x_groups = t.x_groups; P.g_tiles = t.g_tiles;
     // a row stride is a multiple of 16 bytes and below 2^40; one row has none
@@ -647,8 +676,11 @@ extern "C" int agpt_b200_act8_weight_grad(const uint8_t *d_codes, const uint8_t 
     }
     if (tma) pdl_launch(weight_kernel<true>, (unsigned)blocks, WG_THREADS, WG_SMEM, st, P);
     else pdl_launch(weight_kernel<false>, (unsigned)blocks, WG_THREADS, WG_SMEM, st, P);
-    if (t.slices > 1)
-        pdl_launch(weight_finish_kernel, (unsigned)((size + cols + 255) / 256), 256, 0, st, (const float *)P.part, (const float *)P.col_part, t.slices, size, cols, d_weight_grad,
-                   d_bias_grad);
+    if (t.slices > 1) {
+        const int each = t.slices >= SPLIT_FROM ? 128 : 1024;
+        const int64_t weight_blocks = (size + each - 1) / each, bias_blocks = d_bias_grad ? (cols + each - 1) / each : 0;
+        pdl_launch(t.slices >= SPLIT_FROM ? weight_finish_kernel<true> : weight_finish_kernel<false>, (unsigned)(weight_blocks + bias_blocks), 256, 0, st, (const float *)P.part, (const float *)P.col_part, t.slices, size, cols, d_weight_grad,
+                   d_bias_grad, weight_blocks);
+    }
     return launch_status("act8_weight_grad");
 }

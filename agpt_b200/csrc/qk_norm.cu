@@ -24,13 +24,14 @@ struct Rows {                          // queries or keys: heads * head_dim colu
     int64_t ld_x, ld_dy, ld_out;
     const float *gain;                 // NULL: 1
     int wide_out, wide_dy;             // out, dy are float32 (else bfloat16)
+    int heads, groups;                 // groups of lanes per row
 };
 struct Heads {
     Rows q, k;
     const int32_t *pos;
     const float *cosv, *sinv;
     int64_t n;
-    int hq, hk, hd, n_pos, lanes_log2, groups;      // groups of lanes per row, HEADS heads each
+    int hd, n_pos, lanes_log2, groups; // groups of both sides
     float eps;
     vec::Divide by_groups;
     float *partial;                    // backward: [blocks][2][hd]
@@ -49,22 +50,28 @@ template <int VEC> __device__ __forceinline__ void store_either(void *p, int64_t
     if (wide) vec::store<VEC>(reinterpret_cast<float *>(p) + at, v);
     else vec::store<VEC>(reinterpret_cast<bf16 *>(p) + at, v);
 }
-// pair i of VEC elements: cos and sin
-template <int VEC> __device__ __forceinline__ void load_table(const float *p, float (&v)[VEC / 2]) {
+// VEC entries of a table or a gain, by 16 bytes where the rows allow it
+template <int VEC> __device__ __forceinline__ void load_cached(const float *p, float (&v)[VEC]) {
     if constexpr (VEC % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < VEC / 4; i++) {
             const float4 x = __ldg(reinterpret_cast<const float4 *>(p) + i);
-            v[2 * i] = x.x; v[2 * i + 1] = x.z;
+            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC / 2; i++) v[i] = __ldg(p + 2 * i);
+        for (int i = 0; i < VEC; i++) v[i] = __ldg(p + i);
     }
 }
+template <int VEC> __device__ __forceinline__ void load_gain(const float *gain, int c, float (&v)[VEC]) {
+    if (gain) load_cached<VEC>(gain + c, v);
+    else
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[i] = 1.f;
+}
 
-// A group of lanes owns HEADS heads of a row, `groups` apart, so that neighbouring groups read neighbouring heads and the table's entries
-// are read once for HEADS heads; a lane has NV pieces of VEC columns, `lanes` pieces apart.
+// A group of lanes owns HEADS heads of one side of a row, `groups` of that side apart, so that neighbouring groups read neighbouring heads and the table's
+// entries and the gain are read once for HEADS heads; a lane has NV pieces of VEC columns, `lanes` pieces apart.
 template <typename T, int VEC, int NV, int HEADS>
 __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ Heads P) {
     pdl_wait();
@@ -73,31 +80,40 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
     const int64_t task = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> P.lanes_log2;
     const bool live = task < P.tasks;
     const int64_t row = live ? vec::quotient(task, P.by_groups) : 0;
-    const int g = (int)(live ? task - row * P.groups : 0), hd = P.hd, heads = P.hq + P.hk;
+    int g = (int)(live ? task - row * P.groups : 0);
+    const bool is_q = g < P.q.groups;
+    const Rows &m = is_q ? P.q : P.k;
+    if (!is_q) g -= P.q.groups;
+    const int hd = P.hd;
+    const T *x = reinterpret_cast<const T *>(m.x) + row * m.ld_x;
     float v[HEADS][NV][VEC];
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
-        const int h = g + u * P.groups;
-        const bool is_q = h < P.hq;
-        const Rows &m = is_q ? P.q : P.k;
+        const int h = g + u * m.groups;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int c = (lane + k * lanes) * VEC;
-            if (live && h < heads && c < hd) vec::load<VEC>(reinterpret_cast<const T *>(m.x) + row * m.ld_x + (is_q ? h : h - P.hq) * hd + c, v[u][k]);
+            if (live && h < m.heads && c < hd) vec::load<VEC>(x + h * hd + c, v[u][k]);
             else
 #pragma unroll
                 for (int i = 0; i < VEC; i++) v[u][k][i] = 0.f;
         }
     }
-    float cs[NV][VEC / 2], sn[NV][VEC / 2];
+    // entries 2 i of the tables, with the gain of both columns of the pair: y = (x0 r g0) cos - (x1 r g1) sin, (x0 r g0) sin + (x1 r g1) cos
+    float cs[NV][VEC / 2], sn[NV][VEC / 2], gain[NV][VEC];
     const int at = live ? min(max(__ldg(P.pos + row), 0), P.n_pos - 1) : 0;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int c = (lane + k * lanes) * VEC;
-        if (c < hd) {
-            load_table<VEC>(P.cosv + (int64_t)at * hd + c, cs[k]);
-            load_table<VEC>(P.sinv + (int64_t)at * hd + c, sn[k]);
-        }
+        if (c >= hd) continue;
+        float t[VEC];
+        load_cached<VEC>(P.cosv + (int64_t)at * hd + c, t);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) cs[k][i] = t[2 * i];
+        load_cached<VEC>(P.sinv + (int64_t)at * hd + c, t);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) sn[k][i] = t[2 * i];
+        load_gain<VEC>(m.gain, c, gain[k]);
     }
     float r[HEADS];
 #pragma unroll
@@ -112,10 +128,8 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
     if (!live) return;
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
-        const int h = g + u * P.groups;
-        if (h >= heads) break;
-        const bool is_q = h < P.hq;
-        const Rows &m = is_q ? P.q : P.k;
+        const int h = g + u * m.groups;
+        if (h >= m.heads) break;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int c = (lane + k * lanes) * VEC;
@@ -123,49 +137,51 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
             float y[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
-                const float a = v[u][k][i] * r[u] * (m.gain ? __ldg(m.gain + c + i) : 1.f), b = v[u][k][i + 1] * r[u] * (m.gain ? __ldg(m.gain + c + i + 1) : 1.f);
+                const float a = v[u][k][i] * r[u] * gain[k][i], b = v[u][k][i + 1] * r[u] * gain[k][i + 1];
                 y[i] = a * cs[k][i / 2] - b * sn[k][i / 2];
                 y[i + 1] = a * sn[k][i / 2] + b * cs[k][i / 2];
             }
-            store_either<VEC>(m.out, row * m.ld_out + (is_q ? h : h - P.hq) * hd + c, m.wide_out, y);
+            store_either<VEC>(m.out, row * m.ld_out + h * hd + c, m.wide_out, y);
         }
     }
 }
 
-// A thread keeps its columns' gain gradients over all rows of its group; the block adds its groups in order into partial[block].
+// The blocks walk the tasks by a multiple of the groups of a row, so that a thread stays with its heads: side, gain and the columns' gain gradients are its own
+// for the whole kernel, and the row moves by a constant.  The block adds its groups in order into partial[block].
 template <typename T, int VEC, int NV, int HEADS>
-__global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_constant__ Heads P) {
+__global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_constant__ Heads P, const int64_t row_step) {
     pdl_wait();
     pdl_next();
     extern __shared__ float s_gain[];                  // [groups of the block][2][hd]
     const int lanes = 1 << P.lanes_log2, lane = threadIdx.x & (lanes - 1), per_block = 256 >> P.lanes_log2, own = threadIdx.x >> P.lanes_log2;
-    const int hd = P.hd, heads = P.hq + P.hk;
-    float sum[2][NV][VEC];
+    const int hd = P.hd;
+    const int64_t task = (int64_t)blockIdx.x * per_block + own, first = vec::quotient(task, P.by_groups);
+    int g = (int)(task - first * P.groups);
+    const bool is_q = g < P.q.groups;
+    const Rows &m = is_q ? P.q : P.k;
+    if (!is_q) g -= P.q.groups;
+    float sum[NV][VEC], gain[NV][VEC];
 #pragma unroll
-    for (int w = 0; w < 2; w++)
+    for (int k = 0; k < NV; k++) {
+        const int c = (lane + k * lanes) * VEC;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int i = 0; i < VEC; i++) sum[w][k][i] = 0.f;
-    const int64_t rounds = (P.tasks + (int64_t)gridDim.x * per_block - 1) / ((int64_t)gridDim.x * per_block);
+        for (int i = 0; i < VEC; i++) sum[k][i] = gain[k][i] = 0.f;
+        if (c < hd) load_gain<VEC>(m.gain, c, gain[k]);
+    }
+    const int64_t rounds = (P.n + row_step - 1) / row_step;
     for (int64_t t = 0; t < rounds; t++) {
-        const int64_t task = (t * gridDim.x + blockIdx.x) * per_block + own;
-        const bool live = task < P.tasks;
-        const int64_t row = live ? vec::quotient(task, P.by_groups) : 0;
-        const int g = (int)(live ? task - row * P.groups : 0);
+        const int64_t row = first + t * row_step;
+        const bool live = row < P.n;
         float x[HEADS][NV][VEC], d[HEADS][NV][VEC];
 #pragma unroll
         for (int u = 0; u < HEADS; u++) {
-            const int h = g + u * P.groups;
-            const bool is_q = h < P.hq;
-            const Rows &m = is_q ? P.q : P.k;
+            const int h = g + u * m.groups;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 const int c = (lane + k * lanes) * VEC;
-                if (live && h < heads && c < hd) {
-                    const int col = (is_q ? h : h - P.hq) * hd + c;
-                    vec::load<VEC>(reinterpret_cast<const T *>(m.x) + row * m.ld_x + col, x[u][k]);
-                    load_either<VEC>(m.dy, row * m.ld_dy + col, m.wide_dy, d[u][k]);
+                if (live && h < m.heads && c < hd) {
+                    vec::load<VEC>(reinterpret_cast<const T *>(m.x) + row * m.ld_x + h * hd + c, x[u][k]);
+                    load_either<VEC>(m.dy, row * m.ld_dy + h * hd + c, m.wide_dy, d[u][k]);
                 } else
 #pragma unroll
                     for (int i = 0; i < VEC; i++) x[u][k][i] = d[u][k][i] = 0.f;
@@ -176,37 +192,40 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int c = (lane + k * lanes) * VEC;
-            if (c < hd) {
-                load_table<VEC>(P.cosv + (int64_t)at * hd + c, cs[k]);
-                load_table<VEC>(P.sinv + (int64_t)at * hd + c, sn[k]);
-            }
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) cs[k][i] = sn[k][i] = 0.f;
+            if (c >= hd) continue;
+            float e[VEC];
+            load_cached<VEC>(P.cosv + (int64_t)at * hd + c, e);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) cs[k][i] = e[2 * i];
+            load_cached<VEC>(P.sinv + (int64_t)at * hd + c, e);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) sn[k][i] = e[2 * i];
         }
 #pragma unroll
         for (int u = 0; u < HEADS; u++) {
-            const int h = g + u * P.groups;
-            const bool is_q = h < P.hq;
-            const Rows &m = is_q ? P.q : P.k;
-            float sq = 0.f, dot = 0.f, w[NV][VEC];
+            const int h = g + u * m.groups;
+            float sq = 0.f, dot = 0.f;
+            // d becomes w = R^T dy
 #pragma unroll
             for (int k = 0; k < NV; k++) {
-                const int c = (lane + k * lanes) * VEC;
 #pragma unroll
                 for (int i = 0; i < VEC; i += 2) {
-                    const float a = d[u][k][i], b = d[u][k][i + 1], co = c < hd ? cs[k][i / 2] : 0.f, si = c < hd ? sn[k][i / 2] : 0.f;
-                    w[k][i] = a * co + b * si;
-                    w[k][i + 1] = b * co - a * si;
+                    const float a = d[u][k][i], b = d[u][k][i + 1], co = cs[k][i / 2], si = sn[k][i / 2];
+                    d[u][k][i] = a * co + b * si;
+                    d[u][k][i + 1] = b * co - a * si;
                 }
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
                     sq += x[u][k][i] * x[u][k][i];
-                    d[u][k][i] = w[k][i] * (m.gain && c < hd ? __ldg(m.gain + c + i) : 1.f);
-                    dot += d[u][k][i] * x[u][k][i];
+                    dot += d[u][k][i] * gain[k][i] * x[u][k][i];
                 }
             }
             sq = group_sum(sq, lanes);
             dot = group_sum(dot, lanes);
             const float r = 1.f / sqrtf(sq / (float)hd + P.eps), f = r * r * (dot / (float)hd);
-            if (!live || h >= heads) continue;
+            if (!live || h >= m.heads) continue;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 const int c = (lane + k * lanes) * VEC;
@@ -214,24 +233,24 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
                 float y[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
-                    y[i] = r * (d[u][k][i] - x[u][k][i] * f);
-                    const float e = w[k][i] * (x[u][k][i] * r);
-                    if (is_q) sum[0][k][i] += e; else sum[1][k][i] += e;
+                    y[i] = r * (d[u][k][i] * gain[k][i] - x[u][k][i] * f);
+                    sum[k][i] += d[u][k][i] * (x[u][k][i] * r);
                 }
-                store_either<VEC>(m.out, row * m.ld_out + (is_q ? h : h - P.hq) * hd + c, m.wide_out, y);
+                store_either<VEC>(m.out, row * m.ld_out + h * hd + c, m.wide_out, y);
             }
         }
     }
     if (!P.partial) return;
 #pragma unroll
-    for (int w = 0; w < 2; w++)
+    for (int k = 0; k < NV; k++) {
+        const int c = (lane + k * lanes) * VEC;
+        if (c < hd)
 #pragma unroll
-        for (int k = 0; k < NV; k++) {
-            const int c = (lane + k * lanes) * VEC;
-            if (c < hd)
-#pragma unroll
-                for (int i = 0; i < VEC; i++) s_gain[(own * 2 + w) * hd + c + i] = sum[w][k][i];
-        }
+            for (int i = 0; i < VEC; i++) {
+                s_gain[(own * 2 + !is_q) * hd + c + i] = sum[k][i];
+                s_gain[(own * 2 + is_q) * hd + c + i] = 0.f;
+            }
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * hd; c += 256) {
         float s = 0.f;
@@ -270,19 +289,26 @@ bool type_ok(int t) { return t == AGPT_KV_F32 || t == AGPT_KV_BF16; }
 // every row of m starts on a boundary of `vec` elements of its type
 bool rows_aligned(const void *p, int64_t ld, int type, int vec) { return !p || (vec::aligned(p, vec * bytes_of(type) > 16 ? 16 : vec * bytes_of(type)) && ld % vec == 0); }
 
-constexpr int HEADS = 4, BACK_HEADS = 2;
+constexpr int HEADS = 4, BACK_HEADS = 2, MAX_HEADS = 1024;
 
 void split(Heads &P, int vec, int heads_each) {
     const int pieces = (P.hd + vec - 1) / vec;
     P.lanes_log2 = 0;
     while (P.lanes_log2 < 5 && (1 << P.lanes_log2) < pieces) P.lanes_log2++;
-    P.groups = (P.hq + P.hk + heads_each - 1) / heads_each;
+    P.q.groups = (P.q.heads + heads_each - 1) / heads_each;
+    P.k.groups = (P.k.heads + heads_each - 1) / heads_each;
+    P.groups = P.q.groups + P.k.groups;
     P.by_groups = vec::Divide((uint32_t)P.groups);
     P.tasks = P.n * P.groups;
 }
-int backward_blocks(int64_t tasks, int lanes_log2) {
-    const int64_t want = (tasks + (256 >> lanes_log2) - 1) / (256 >> lanes_log2), most = (int64_t)vec::sm_count() * 4;
-    return (int)(want < most ? want : most);
+// Blocks of the backward: as many as run at once, in a number that makes their tasks a multiple of the groups of a row.
+int64_t most_blocks() { return (int64_t)vec::sm_count() * 4; }
+int backward_blocks(const Heads &P) {
+    const int per_block = 256 >> P.lanes_log2;
+    int step = P.groups;                               // groups / gcd(groups, per_block), per_block a power of two
+    for (int b = per_block; b > 1 && step % 2 == 0; b /= 2) step /= 2;
+    const int64_t want = (P.tasks + per_block - 1) / per_block, rounded = (want + step - 1) / step * step, most = most_blocks() / step * step;
+    return (int)(rounded < most ? rounded : most < step ? step : most);
 }
 
 template <typename T, int VEC, int NV>
@@ -296,16 +322,16 @@ int forward(Heads &P, cudaStream_t st) {
 template <typename T, int VEC, int NV>
 int backward(Heads &P, float *dq_gain, float *dk_gain, cudaStream_t st) {
     split(P, VEC, BACK_HEADS);
-    const int blocks = backward_blocks(P.tasks, P.lanes_log2);
-    const size_t smem = P.partial ? (size_t)(256 >> P.lanes_log2) * 2 * P.hd * 4 : 0;
-    pdl_launch(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS>, (unsigned)blocks, 256, smem, st, P);
+    const int blocks = backward_blocks(P), per_block = 256 >> P.lanes_log2;
+    const size_t smem = P.partial ? (size_t)per_block * 2 * P.hd * 4 : 0;
+    pdl_launch(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS>, (unsigned)blocks, 256, smem, st, P, (int64_t)blocks * per_block / P.groups);
     if (P.partial) pdl_launch(gain_finish_kernel, (unsigned)((2 * P.hd + 31) / 32), 256, 0, st, (const float *)P.partial, blocks, P.hd, dq_gain, dk_gain);
     return launch_status("qk_norm_rope_backward");
 }
 
 int check(const char *who, int64_t n, int hq, int hk, int hd, int n_pos, int x_type, int64_t q_ld, int64_t k_ld, float eps) {
     if (n < 0 || hq < 1 || hk < 1 || hd < 2 || hd % 2 || n_pos < 1 || !type_ok(x_type) || !(eps > 0.f)) return agpt_set_error(AGPT_E_ARG, "%s: bad argument", who);
-    if (hd > 256 || hq + hk > 1024) return agpt_set_error(AGPT_E_LIMIT, "%s: head_dim up to 256 and 1024 heads", who);
+    if (hd > 256 || hq + hk > MAX_HEADS) return agpt_set_error(AGPT_E_LIMIT, "%s: head_dim up to 256 and 1024 heads", who);
     if (n > (int64_t)1 << 40) return agpt_set_error(AGPT_E_LIMIT, "%s: too many rows", who);
     if (q_ld < (int64_t)hq * hd || k_ld < (int64_t)hk * hd) return agpt_set_error(AGPT_E_ARG, "%s: rows overlap", who);
     return AGPT_OK;
@@ -321,13 +347,13 @@ extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void 
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad output type or stride");
     if (n == 0) return AGPT_OK;
     if (!d_q || !d_k || !d_pos || !d_cos || !d_sin || !d_q_out || !d_k_out) return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad argument");
-    Heads P{{d_q, nullptr, d_q_out, q_ld, 0, q_out_ld, d_q_gain, q_out_type == AGPT_KV_F32, 0},
-            {d_k, nullptr, d_k_out, k_ld, 0, k_out_ld, d_k_gain, k_out_type == AGPT_KV_F32, 0},
-            d_pos, d_cos, d_sin, n, q_heads, k_heads, head_dim, n_pos, 0, 0, eps, vec::Divide(1), nullptr, 0};
+    Heads P{{d_q, nullptr, d_q_out, q_ld, 0, q_out_ld, d_q_gain, q_out_type == AGPT_KV_F32, 0, q_heads, 0},
+            {d_k, nullptr, d_k_out, k_ld, 0, k_out_ld, d_k_gain, k_out_type == AGPT_KV_F32, 0, k_heads, 0},
+            d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, vec::Divide(1), nullptr, 0};
     cudaStream_t st = (cudaStream_t)stream;
     const auto fits = [&](int v) {
         return head_dim % v == 0 && rows_aligned(d_q, q_ld, type, v) && rows_aligned(d_k, k_ld, type, v) && rows_aligned(d_q_out, q_out_ld, q_out_type, v) &&
-               rows_aligned(d_k_out, k_out_ld, k_out_type, v) && vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16);
+               rows_aligned(d_k_out, k_out_ld, k_out_type, v) && vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16) && vec::aligned(d_q_gain, 16) && vec::aligned(d_k_gain, 16);
     };
     if (type == AGPT_KV_BF16) return fits(8) ? forward<bf16, 8, 1>(P, st) : forward<bf16, 2, 4>(P, st);
     if (!fits(4)) return forward<float, 2, 4>(P, st);
@@ -336,7 +362,7 @@ extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void 
 
 extern "C" int64_t agpt_b200_qk_norm_rope_backward_workspace_bytes(int head_dim) {
     if (head_dim < 2 || head_dim > 256) return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward_workspace_bytes: bad argument");
-    return (int64_t)vec::sm_count() * 4 * 2 * head_dim * 4;
+    return (most_blocks() + MAX_HEADS) * 2 * head_dim * 4;
 }
 
 extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, const void *d_dk, int64_t dk_ld, int grad_type, const void *d_q, int64_t q_ld,
@@ -353,13 +379,13 @@ extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, 
     if (gains && (!d_workspace || workspace_bytes < agpt_b200_qk_norm_rope_backward_workspace_bytes(head_dim) || !vec::aligned(d_workspace, 16)))
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward: workspace too small (agpt_b200_qk_norm_rope_backward_workspace_bytes)");
     const int wide = type == AGPT_KV_F32, wide_dy = grad_type == AGPT_KV_F32;
-    Heads P{{d_q, d_dq, d_q_out, q_ld, dq_ld, q_out_ld, d_q_gain, wide, wide_dy}, {d_k, d_dk, d_k_out, k_ld, dk_ld, k_out_ld, d_k_gain, wide, wide_dy},
-            d_pos, d_cos, d_sin, n, q_heads, k_heads, head_dim, n_pos, 0, 0, eps, vec::Divide(1), gains ? (float *)d_workspace : nullptr, 0};
+    Heads P{{d_q, d_dq, d_q_out, q_ld, dq_ld, q_out_ld, d_q_gain, wide, wide_dy, q_heads, 0}, {d_k, d_dk, d_k_out, k_ld, dk_ld, k_out_ld, d_k_gain, wide, wide_dy, k_heads, 0},
+            d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, vec::Divide(1), gains ? (float *)d_workspace : nullptr, 0};
     cudaStream_t st = (cudaStream_t)stream;
     const auto fits = [&](int v) {
         return head_dim % v == 0 && rows_aligned(d_q, q_ld, type, v) && rows_aligned(d_k, k_ld, type, v) && rows_aligned(d_q_out, q_out_ld, type, v) &&
                rows_aligned(d_k_out, k_out_ld, type, v) && rows_aligned(d_dq, dq_ld, grad_type, v) && rows_aligned(d_dk, dk_ld, grad_type, v) &&
-               vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16);
+               vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16) && vec::aligned(d_q_gain, 16) && vec::aligned(d_k_gain, 16);
     };
     if (type == AGPT_KV_BF16)
         return fits(8) ? backward<bf16, 8, 1>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<bf16, 2, 4>(P, d_q_gain_grad, d_k_gain_grad, st);
