@@ -32,14 +32,20 @@ struct Heads {
     const float *cosv, *sinv;
     int64_t n;
     int hd, n_pos, lanes_log2, groups; // groups of both sides
-    float eps;
+    float eps, inv_hd;                 // 1 / hd: exact for powers of two, else one rounding
     vec::Divide by_groups;
     float *partial;                    // backward: [blocks][2][hd]
     int64_t tasks;
 };
 
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// LOG2 >= 0: the lanes of a group are known to the compiler
+template <int LOG2> __device__ __forceinline__ float group_sum(float v, int lanes) {
+    if constexpr (LOG2 >= 0) {
+#pragma unroll
+        for (int o = (1 << LOG2) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    } else {
+        for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
     return v;
 }
 template <int VEC> __device__ __forceinline__ void load_either(const void *p, int64_t at, int wide, float (&v)[VEC]) {
@@ -72,12 +78,12 @@ template <int VEC> __device__ __forceinline__ void load_gain(const float *gain, 
 
 // A group of lanes owns HEADS heads of one side of a row, `groups` of that side apart, so that neighbouring groups read neighbouring heads and the table's
 // entries and the gain are read once for HEADS heads; a lane has NV pieces of VEC columns, `lanes` pieces apart.
-template <typename T, int VEC, int NV, int HEADS>
+template <typename T, int VEC, int NV, int HEADS, int LOG2>
 __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ Heads P) {
     pdl_wait();
     pdl_next();
-    const int lanes = 1 << P.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const int64_t task = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> P.lanes_log2;
+    const int lanes_log2 = LOG2 >= 0 ? LOG2 : P.lanes_log2, lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const int64_t task = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lanes_log2;
     const bool live = task < P.tasks;
     const int64_t row = live ? vec::quotient(task, P.by_groups) : 0;
     int g = (int)(live ? task - row * P.groups : 0);
@@ -123,7 +129,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int i = 0; i < VEC; i++) s += v[u][k][i] * v[u][k][i];
-        r[u] = 1.f / sqrtf(group_sum(s, lanes) / (float)hd + P.eps);
+        r[u] = rsqrtf(group_sum<LOG2>(s, lanes) * P.inv_hd + P.eps);
     }
     if (!live) return;
 #pragma unroll
@@ -148,12 +154,13 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
 
 // The blocks walk the tasks by a multiple of the groups of a row, so that a thread stays with its heads: side, gain and the columns' gain gradients are its own
 // for the whole kernel, and the row moves by a constant.  The block adds its groups in order into partial[block].
-template <typename T, int VEC, int NV, int HEADS>
+template <typename T, int VEC, int NV, int HEADS, int LOG2>
 __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_constant__ Heads P, const int64_t row_step) {
     pdl_wait();
     pdl_next();
     extern __shared__ float s_gain[];                  // [groups of the block][2][hd]
-    const int lanes = 1 << P.lanes_log2, lane = threadIdx.x & (lanes - 1), per_block = 256 >> P.lanes_log2, own = threadIdx.x >> P.lanes_log2;
+    const int lanes_log2 = LOG2 >= 0 ? LOG2 : P.lanes_log2, lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), per_block = 256 >> lanes_log2,
+              own = threadIdx.x >> lanes_log2;
     const int hd = P.hd;
     const int64_t task = (int64_t)blockIdx.x * per_block + own, first = vec::quotient(task, P.by_groups);
     int g = (int)(task - first * P.groups);
@@ -222,9 +229,9 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
                     dot += d[u][k][i] * gain[k][i] * x[u][k][i];
                 }
             }
-            sq = group_sum(sq, lanes);
-            dot = group_sum(dot, lanes);
-            const float r = 1.f / sqrtf(sq / (float)hd + P.eps), f = r * r * (dot / (float)hd);
+            sq = group_sum<LOG2>(sq, lanes);
+            dot = group_sum<LOG2>(dot, lanes);
+            const float r = rsqrtf(sq * P.inv_hd + P.eps), f = r * r * (dot * P.inv_hd);
             if (!live || h >= m.heads) continue;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
@@ -259,20 +266,22 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
     }
 }
 
-// dq_gain, dk_gain += the blocks' sums: a block has 32 columns, its eight warps a run of the blocks each
-__global__ void __launch_bounds__(256) gain_finish_kernel(const float *__restrict__ partial, int blocks, int hd, float *__restrict__ dq_gain, float *__restrict__ dk_gain) {
+// dq_gain, dk_gain += the blocks' sums: a block has eight columns (a 32-byte sector), a thread a column and a 64th of the blocks
+constexpr int FINISH_COLS = 8, FINISH_RUNS = 64;
+__global__ void __launch_bounds__(FINISH_COLS *FINISH_RUNS) gain_finish_kernel(const float *__restrict__ partial, int blocks, int hd, float *__restrict__ dq_gain,
+                                                                               float *__restrict__ dk_gain) {
     pdl_wait();
     pdl_next();
-    __shared__ float s[8][32];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    __shared__ float s[FINISH_RUNS][FINISH_COLS];
+    const int col = threadIdx.x % FINISH_COLS, run = threadIdx.x / FINISH_COLS, c = blockIdx.x * FINISH_COLS + col;
     float t = 0.f;
     if (c < 2 * hd)
-#pragma unroll 8
-        for (int b = blocks * w / 8; b < blocks * (w + 1) / 8; b++) t += partial[(int64_t)b * 2 * hd + c];
-    s[w][lane] = t;
+#pragma unroll 16
+        for (int b = blocks * run / FINISH_RUNS; b < blocks * (run + 1) / FINISH_RUNS; b++) t += partial[(int64_t)b * 2 * hd + c];
+    s[run][col] = t;
     __syncthreads();
-    if (w || c >= 2 * hd) return;
-    for (int k = 1; k < 8; k++) t += s[k][lane];
+    if (run || c >= 2 * hd) return;
+    for (int k = 1; k < FINISH_RUNS; k++) t += s[k][col];
     float *to = c < hd ? dq_gain : dk_gain;
     if (to) to[c < hd ? c : c - hd] += t;
 }
@@ -291,9 +300,9 @@ bool rows_aligned(const void *p, int64_t ld, int type, int vec) { return !p || (
 
 constexpr int HEADS = 4, BACK_HEADS = 2, MAX_HEADS = 1024;
 
-void split(Heads &P, int vec, int heads_each) {
+void split(Heads &P, int vec, int heads_each, int low) {
     const int pieces = (P.hd + vec - 1) / vec;
-    P.lanes_log2 = 0;
+    P.lanes_log2 = low < 0 ? 0 : low;
     while (P.lanes_log2 < 5 && (1 << P.lanes_log2) < pieces) P.lanes_log2++;
     P.q.groups = (P.q.heads + heads_each - 1) / heads_each;
     P.k.groups = (P.k.heads + heads_each - 1) / heads_each;
@@ -311,21 +320,39 @@ int backward_blocks(const Heads &P) {
     return (int)(rounded < most ? rounded : most < step ? step : most);
 }
 
-template <typename T, int VEC, int NV>
+// kernel by the lanes of a group (down to 2^LOW; narrower heads leave lanes idle)
+template <typename T, int VEC, int NV, int LOW>
 int forward(Heads &P, cudaStream_t st) {
-    split(P, VEC, HEADS);
+    split(P, VEC, HEADS, LOW);
     const int64_t blocks = ((P.tasks << P.lanes_log2) + 255) / 256;
     if (blocks > INT32_MAX) return agpt_set_error(AGPT_E_LIMIT, "qk_norm_rope: too many rows");
-    pdl_launch(norm_rope_kernel<T, VEC, NV, HEADS>, (unsigned)blocks, 256, 0, st, P);
+    const auto go = [&](void (*kernel)(const Heads)) { pdl_launch(kernel, (unsigned)blocks, 256, 0, st, P); };
+    if constexpr (LOW < 0) go(norm_rope_kernel<T, VEC, NV, HEADS, -1>);
+    else switch (P.lanes_log2) {
+        case 5: go(norm_rope_kernel<T, VEC, NV, HEADS, 5>); break;
+        case 4: go(norm_rope_kernel<T, VEC, NV, HEADS, LOW < 4 ? 4 : LOW>); break;
+        case 3: go(norm_rope_kernel<T, VEC, NV, HEADS, LOW < 3 ? 3 : LOW>); break;
+        case 2: go(norm_rope_kernel<T, VEC, NV, HEADS, LOW < 2 ? 2 : LOW>); break;
+        default: go(norm_rope_kernel<T, VEC, NV, HEADS, LOW>);
+    }
     return launch_status("qk_norm_rope");
 }
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, int LOW>
 int backward(Heads &P, float *dq_gain, float *dk_gain, cudaStream_t st) {
-    split(P, VEC, BACK_HEADS);
+    split(P, VEC, BACK_HEADS, LOW);
     const int blocks = backward_blocks(P), per_block = 256 >> P.lanes_log2;
     const size_t smem = P.partial ? (size_t)per_block * 2 * P.hd * 4 : 0;
-    pdl_launch(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS>, (unsigned)blocks, 256, smem, st, P, (int64_t)blocks * per_block / P.groups);
-    if (P.partial) pdl_launch(gain_finish_kernel, (unsigned)((2 * P.hd + 31) / 32), 256, 0, st, (const float *)P.partial, blocks, P.hd, dq_gain, dk_gain);
+    const int64_t row_step = (int64_t)blocks * per_block / P.groups;
+    const auto go = [&](void (*kernel)(const Heads, const int64_t)) { pdl_launch(kernel, (unsigned)blocks, 256, smem, st, P, row_step); };
+    if constexpr (LOW < 0) go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, -1>);
+    else switch (P.lanes_log2) {
+        case 5: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, 5>); break;
+        case 4: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW < 4 ? 4 : LOW>); break;
+        case 3: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW < 3 ? 3 : LOW>); break;
+        case 2: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW < 2 ? 2 : LOW>); break;
+        default: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW>);
+    }
+    if (P.partial) pdl_launch(gain_finish_kernel, (unsigned)((2 * P.hd + FINISH_COLS - 1) / FINISH_COLS), FINISH_COLS * FINISH_RUNS, 0, st, (const float *)P.partial, blocks, P.hd, dq_gain, dk_gain);
     return launch_status("qk_norm_rope_backward");
 }
 
@@ -349,15 +376,15 @@ extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void 
     if (!d_q || !d_k || !d_pos || !d_cos || !d_sin || !d_q_out || !d_k_out) return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad argument");
     Heads P{{d_q, nullptr, d_q_out, q_ld, 0, q_out_ld, d_q_gain, q_out_type == AGPT_KV_F32, 0, q_heads, 0},
             {d_k, nullptr, d_k_out, k_ld, 0, k_out_ld, d_k_gain, k_out_type == AGPT_KV_F32, 0, k_heads, 0},
-            d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, vec::Divide(1), nullptr, 0};
+            d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, 1.f / (float)head_dim, vec::Divide(1), nullptr, 0};
     cudaStream_t st = (cudaStream_t)stream;
     const auto fits = [&](int v) {
         return head_dim % v == 0 && rows_aligned(d_q, q_ld, type, v) && rows_aligned(d_k, k_ld, type, v) && rows_aligned(d_q_out, q_out_ld, q_out_type, v) &&
                rows_aligned(d_k_out, k_out_ld, k_out_type, v) && vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16) && vec::aligned(d_q_gain, 16) && vec::aligned(d_k_gain, 16);
     };
-    if (type == AGPT_KV_BF16) return fits(8) ? forward<bf16, 8, 1>(P, st) : forward<bf16, 2, 4>(P, st);
-    if (!fits(4)) return forward<float, 2, 4>(P, st);
-    return head_dim <= 128 ? forward<float, 4, 1>(P, st) : forward<float, 4, 2>(P, st);
+    if (type == AGPT_KV_BF16) return fits(8) ? forward<bf16, 8, 1, 1>(P, st) : forward<bf16, 2, 4, -1>(P, st);
+    if (!fits(4)) return forward<float, 2, 4, -1>(P, st);
+    return head_dim <= 128 ? forward<float, 4, 1, 2>(P, st) : forward<float, 4, 2, 5>(P, st);
 }
 
 extern "C" int64_t agpt_b200_qk_norm_rope_backward_workspace_bytes(int head_dim) {
@@ -380,7 +407,7 @@ extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, 
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward: workspace too small (agpt_b200_qk_norm_rope_backward_workspace_bytes)");
     const int wide = type == AGPT_KV_F32, wide_dy = grad_type == AGPT_KV_F32;
     Heads P{{d_q, d_dq, d_q_out, q_ld, dq_ld, q_out_ld, d_q_gain, wide, wide_dy, q_heads, 0}, {d_k, d_dk, d_k_out, k_ld, dk_ld, k_out_ld, d_k_gain, wide, wide_dy, k_heads, 0},
-            d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, vec::Divide(1), gains ? (float *)d_workspace : nullptr, 0};
+            d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, 1.f / (float)head_dim, vec::Divide(1), gains ? (float *)d_workspace : nullptr, 0};
     cudaStream_t st = (cudaStream_t)stream;
     const auto fits = [&](int v) {
         return head_dim % v == 0 && rows_aligned(d_q, q_ld, type, v) && rows_aligned(d_k, k_ld, type, v) && rows_aligned(d_q_out, q_out_ld, type, v) &&
@@ -388,7 +415,7 @@ extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, 
                vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16) && vec::aligned(d_q_gain, 16) && vec::aligned(d_k_gain, 16);
     };
     if (type == AGPT_KV_BF16)
-        return fits(8) ? backward<bf16, 8, 1>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<bf16, 2, 4>(P, d_q_gain_grad, d_k_gain_grad, st);
-    if (!fits(4)) return backward<float, 2, 4>(P, d_q_gain_grad, d_k_gain_grad, st);
-    return head_dim <= 128 ? backward<float, 4, 1>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<float, 4, 2>(P, d_q_gain_grad, d_k_gain_grad, st);
+        return fits(8) ? backward<bf16, 8, 1, 1>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<bf16, 2, 4, -1>(P, d_q_gain_grad, d_k_gain_grad, st);
+    if (!fits(4)) return backward<float, 2, 4, -1>(P, d_q_gain_grad, d_k_gain_grad, st);
+    return head_dim <= 128 ? backward<float, 4, 1, 2>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<float, 4, 2, 5>(P, d_q_gain_grad, d_k_gain_grad, st);
 }
