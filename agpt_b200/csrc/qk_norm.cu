@@ -18,12 +18,14 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
+constexpr int BACK_BLOCKS = 3;         // blocks of the backward on an SM
+
 struct Rows {                          // queries or keys: heads * head_dim columns, rows ld elements apart
     const void *x, *dy;
     void *out;                         // y, or dx
     int64_t ld_x, ld_dy, ld_out;
     const float *gain;                 // NULL: 1
-    int wide_out, wide_dy;             // out, dy are float32 (else bfloat16)
+    int wide_out;                      // out is float32 (else bfloat16)
     int heads, groups;                 // groups of lanes per row
 };
 struct Heads {
@@ -47,10 +49,6 @@ template <int LOG2> __device__ __forceinline__ float group_sum(float v, int lane
         for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
     return v;
-}
-template <int VEC> __device__ __forceinline__ void load_either(const void *p, int64_t at, int wide, float (&v)[VEC]) {
-    if (wide) vec::load<VEC>(reinterpret_cast<const float *>(p) + at, v);
-    else vec::load<VEC>(reinterpret_cast<const bf16 *>(p) + at, v);
 }
 template <int VEC> __device__ __forceinline__ void store_either(void *p, int64_t at, int wide, const float (&v)[VEC]) {
     if (wide) vec::store<VEC>(reinterpret_cast<float *>(p) + at, v);
@@ -92,17 +90,14 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
     if (!is_q) g -= P.q.groups;
     const int hd = P.hd;
     const T *x = reinterpret_cast<const T *>(m.x) + row * m.ld_x;
-    float v[HEADS][NV][VEC];
+    vec::Piece<T, VEC> piece[HEADS][NV];
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
         const int h = g + u * m.groups;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int c = (lane + k * lanes) * VEC;
-            if (live && h < m.heads && c < hd) vec::load<VEC>(x + h * hd + c, v[u][k]);
-            else
-#pragma unroll
-                for (int i = 0; i < VEC; i++) v[u][k][i] = 0.f;
+            piece[u][k].fetch(x + h * hd + c, live && h < m.heads && c < hd);
         }
     }
     // entries 2 i of the tables, with the gain of both columns of the pair: y = (x0 r g0) cos - (x1 r g1) sin, (x0 r g0) sin + (x1 r g1) cos
@@ -121,14 +116,16 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
         for (int i = 0; i < VEC / 2; i++) sn[k][i] = t[2 * i];
         load_gain<VEC>(m.gain, c, gain[k]);
     }
-    float r[HEADS];
+    float r[HEADS], v[HEADS][NV][VEC];
 #pragma unroll
     for (int u = 0; u < HEADS; u++) {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < NV; k++)
+        for (int k = 0; k < NV; k++) {
+            piece[u][k].values(v[u][k]);
 #pragma unroll
             for (int i = 0; i < VEC; i++) s += v[u][k][i] * v[u][k][i];
+        }
         r[u] = rsqrtf(group_sum<LOG2>(s, lanes) * P.inv_hd + P.eps);
     }
     if (!live) return;
@@ -154,8 +151,8 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
 
 // The blocks walk the tasks by a multiple of the groups of a row, so that a thread stays with its heads: side, gain and the columns' gain gradients are its own
 // for the whole kernel, and the row moves by a constant.  The block adds its groups in order into partial[block].
-template <typename T, int VEC, int NV, int HEADS, int LOG2>
-__global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_constant__ Heads P, const int64_t row_step) {
+template <typename T, typename D, int VEC, int NV, int HEADS, int LOG2>
+__global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_backward_kernel(const __grid_constant__ Heads P, const int64_t row_step) {
     pdl_wait();
     pdl_next();
     extern __shared__ float s_gain[];                  // [groups of the block][2][hd]
@@ -179,19 +176,18 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
     for (int64_t t = 0; t < rounds; t++) {
         const int64_t row = first + t * row_step;
         const bool live = row < P.n;
-        float x[HEADS][NV][VEC], d[HEADS][NV][VEC];
+        vec::Piece<T, VEC> x_piece[HEADS][NV];
+        vec::Piece<D, VEC> d_piece[HEADS][NV];
+        const T *at_x = reinterpret_cast<const T *>(m.x) + row * m.ld_x;
+        const D *at_d = reinterpret_cast<const D *>(m.dy) + row * m.ld_dy;
 #pragma unroll
         for (int u = 0; u < HEADS; u++) {
             const int h = g + u * m.groups;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 const int c = (lane + k * lanes) * VEC;
-                if (live && h < m.heads && c < hd) {
-                    vec::load<VEC>(reinterpret_cast<const T *>(m.x) + row * m.ld_x + h * hd + c, x[u][k]);
-                    load_either<VEC>(m.dy, row * m.ld_dy + h * hd + c, m.wide_dy, d[u][k]);
-                } else
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) x[u][k][i] = d[u][k][i] = 0.f;
+                x_piece[u][k].fetch(at_x + h * hd + c, live && h < m.heads && c < hd);
+                d_piece[u][k].fetch(at_d + h * hd + c, live && h < m.heads && c < hd);
             }
         }
         const int at = live ? min(max(__ldg(P.pos + row), 0), P.n_pos - 1) : 0;
@@ -213,20 +209,22 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
 #pragma unroll
         for (int u = 0; u < HEADS; u++) {
             const int h = g + u * m.groups;
-            float sq = 0.f, dot = 0.f;
+            float sq = 0.f, dot = 0.f, x[NV][VEC], d[NV][VEC];
             // d becomes w = R^T dy
 #pragma unroll
             for (int k = 0; k < NV; k++) {
+                x_piece[u][k].values(x[k]);
+                d_piece[u][k].values(d[k]);
 #pragma unroll
                 for (int i = 0; i < VEC; i += 2) {
-                    const float a = d[u][k][i], b = d[u][k][i + 1], co = cs[k][i / 2], si = sn[k][i / 2];
-                    d[u][k][i] = a * co + b * si;
-                    d[u][k][i + 1] = b * co - a * si;
+                    const float a = d[k][i], b = d[k][i + 1], co = cs[k][i / 2], si = sn[k][i / 2];
+                    d[k][i] = a * co + b * si;
+                    d[k][i + 1] = b * co - a * si;
                 }
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
-                    sq += x[u][k][i] * x[u][k][i];
-                    dot += d[u][k][i] * gain[k][i] * x[u][k][i];
+                    sq += x[k][i] * x[k][i];
+                    dot += d[k][i] * gain[k][i] * x[k][i];
                 }
             }
             sq = group_sum<LOG2>(sq, lanes);
@@ -240,8 +238,8 @@ __global__ void __launch_bounds__(256) norm_rope_backward_kernel(const __grid_co
                 float y[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
-                    y[i] = r * (d[u][k][i] * gain[k][i] - x[u][k][i] * f);
-                    sum[k][i] += d[u][k][i] * (x[u][k][i] * r);
+                    y[i] = r * (d[k][i] * gain[k][i] - x[k][i] * f);
+                    sum[k][i] += d[k][i] * (x[k][i] * r);
                 }
                 store_either<VEC>(m.out, row * m.ld_out + h * hd + c, m.wide_out, y);
             }
@@ -311,7 +309,7 @@ void split(Heads &P, int vec, int heads_each, int low) {
     P.tasks = P.n * P.groups;
 }
 // Blocks of the backward: as many as run at once, in a number that makes their tasks a multiple of the groups of a row.
-int64_t most_blocks() { return (int64_t)vec::sm_count() * 4; }
+int64_t most_blocks() { return (int64_t)vec::sm_count() * BACK_BLOCKS; }
 int backward_blocks(const Heads &P) {
     const int per_block = 256 >> P.lanes_log2;
     int step = P.groups;                               // groups / gcd(groups, per_block), per_block a power of two
@@ -337,20 +335,20 @@ int forward(Heads &P, cudaStream_t st) {
     }
     return launch_status("qk_norm_rope");
 }
-template <typename T, int VEC, int NV, int LOW>
+template <typename T, typename D, int VEC, int NV, int LOW>
 int backward(Heads &P, float *dq_gain, float *dk_gain, cudaStream_t st) {
     split(P, VEC, BACK_HEADS, LOW);
     const int blocks = backward_blocks(P), per_block = 256 >> P.lanes_log2;
     const size_t smem = P.partial ? (size_t)per_block * 2 * P.hd * 4 : 0;
     const int64_t row_step = (int64_t)blocks * per_block / P.groups;
     const auto go = [&](void (*kernel)(const Heads, const int64_t)) { pdl_launch(kernel, (unsigned)blocks, 256, smem, st, P, row_step); };
-    if constexpr (LOW < 0) go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, -1>);
+    if constexpr (LOW < 0) go(norm_rope_backward_kernel<T, D, VEC, NV, BACK_HEADS, -1>);
     else switch (P.lanes_log2) {
-        case 5: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, 5>); break;
-        case 4: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW < 4 ? 4 : LOW>); break;
-        case 3: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW < 3 ? 3 : LOW>); break;
-        case 2: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW < 2 ? 2 : LOW>); break;
-        default: go(norm_rope_backward_kernel<T, VEC, NV, BACK_HEADS, LOW>);
+        case 5: go(norm_rope_backward_kernel<T, D, VEC, NV, BACK_HEADS, 5>); break;
+        case 4: go(norm_rope_backward_kernel<T, D, VEC, NV, BACK_HEADS, LOW < 4 ? 4 : LOW>); break;
+        case 3: go(norm_rope_backward_kernel<T, D, VEC, NV, BACK_HEADS, LOW < 3 ? 3 : LOW>); break;
+        case 2: go(norm_rope_backward_kernel<T, D, VEC, NV, BACK_HEADS, LOW < 2 ? 2 : LOW>); break;
+        default: go(norm_rope_backward_kernel<T, D, VEC, NV, BACK_HEADS, LOW>);
     }
     if (P.partial) pdl_launch(gain_finish_kernel, (unsigned)((2 * P.hd + FINISH_COLS - 1) / FINISH_COLS), FINISH_COLS * FINISH_RUNS, 0, st, (const float *)P.partial, blocks, P.hd, dq_gain, dk_gain);
     return launch_status("qk_norm_rope_backward");
@@ -374,8 +372,8 @@ extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void 
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad output type or stride");
     if (n == 0) return AGPT_OK;
     if (!d_q || !d_k || !d_pos || !d_cos || !d_sin || !d_q_out || !d_k_out) return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad argument");
-    Heads P{{d_q, nullptr, d_q_out, q_ld, 0, q_out_ld, d_q_gain, q_out_type == AGPT_KV_F32, 0, q_heads, 0},
-            {d_k, nullptr, d_k_out, k_ld, 0, k_out_ld, d_k_gain, k_out_type == AGPT_KV_F32, 0, k_heads, 0},
+    Heads P{{d_q, nullptr, d_q_out, q_ld, 0, q_out_ld, d_q_gain, q_out_type == AGPT_KV_F32, q_heads, 0},
+            {d_k, nullptr, d_k_out, k_ld, 0, k_out_ld, d_k_gain, k_out_type == AGPT_KV_F32, k_heads, 0},
             d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, 1.f / (float)head_dim, vec::Divide(1), nullptr, 0};
     cudaStream_t st = (cudaStream_t)stream;
     const auto fits = [&](int v) {
@@ -406,7 +404,7 @@ extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, 
     if (gains && (!d_workspace || workspace_bytes < agpt_b200_qk_norm_rope_backward_workspace_bytes(head_dim) || !vec::aligned(d_workspace, 16)))
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward: workspace too small (agpt_b200_qk_norm_rope_backward_workspace_bytes)");
     const int wide = type == AGPT_KV_F32, wide_dy = grad_type == AGPT_KV_F32;
-    Heads P{{d_q, d_dq, d_q_out, q_ld, dq_ld, q_out_ld, d_q_gain, wide, wide_dy, q_heads, 0}, {d_k, d_dk, d_k_out, k_ld, dk_ld, k_out_ld, d_k_gain, wide, wide_dy, k_heads, 0},
+    Heads P{{d_q, d_dq, d_q_out, q_ld, dq_ld, q_out_ld, d_q_gain, wide, q_heads, 0}, {d_k, d_dk, d_k_out, k_ld, dk_ld, k_out_ld, d_k_gain, wide, k_heads, 0},
             d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, 1.f / (float)head_dim, vec::Divide(1), gains ? (float *)d_workspace : nullptr, 0};
     cudaStream_t st = (cudaStream_t)stream;
     const auto fits = [&](int v) {
@@ -414,8 +412,14 @@ extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, 
                rows_aligned(d_k_out, k_out_ld, type, v) && rows_aligned(d_dq, dq_ld, grad_type, v) && rows_aligned(d_dk, dk_ld, grad_type, v) &&
                vec::aligned(d_cos, 16) && vec::aligned(d_sin, 16) && vec::aligned(d_q_gain, 16) && vec::aligned(d_k_gain, 16);
     };
-    if (type == AGPT_KV_BF16)
-        return fits(8) ? backward<bf16, 8, 1, 1>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<bf16, 2, 4, -1>(P, d_q_gain_grad, d_k_gain_grad, st);
-    if (!fits(4)) return backward<float, 2, 4, -1>(P, d_q_gain_grad, d_k_gain_grad, st);
-    return head_dim <= 128 ? backward<float, 4, 1, 2>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<float, 4, 2, 5>(P, d_q_gain_grad, d_k_gain_grad, st);
+    const auto run = [&](auto x, auto dy) {
+        using T = decltype(x);
+        using D = decltype(dy);
+        if constexpr (sizeof(T) == 2)
+            return fits(8) ? backward<T, D, 8, 1, 1>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<T, D, 2, 4, -1>(P, d_q_gain_grad, d_k_gain_grad, st);
+        else if (!fits(4)) return backward<T, D, 2, 4, -1>(P, d_q_gain_grad, d_k_gain_grad, st);
+        else return head_dim <= 128 ? backward<T, D, 4, 1, 2>(P, d_q_gain_grad, d_k_gain_grad, st) : backward<T, D, 4, 2, 5>(P, d_q_gain_grad, d_k_gain_grad, st);
+    };
+    if (wide) return wide_dy ? run(0.f, 0.f) : run(0.f, bf16());
+    return wide_dy ? run(bf16(), 0.f) : run(bf16(), bf16());
 }

@@ -60,6 +60,51 @@ template <int VEC> __device__ __forceinline__ void store(__nv_bfloat16 *p, const
     }
 }
 
+// The same in two steps, so that many loads are on their way before the first value is asked for: fetch() is one predicated load without a branch (zeros where it
+// is not wanted), values() turns what came into floats.  A conversion behind a guarded load would make each load wait for the one before.
+template <typename T, int VEC> struct Piece {
+    static constexpr int WORDS = VEC * (int)sizeof(T) / 4, N = WORDS > 0 ? WORDS : 1;
+    uint32_t w[N];
+    __device__ __forceinline__ void fetch(const T *p, bool wanted) {
+        if constexpr (WORDS >= 4) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4)
+                asm volatile("{ .reg .pred p; setp.ne.u32 p, %5, 0; mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0; @p ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4]; }"
+                             : "=&r"(w[i]), "=&r"(w[i + 1]), "=&r"(w[i + 2]), "=&r"(w[i + 3]) : "l"(reinterpret_cast<const uint32_t *>(p) + i), "r"((uint32_t)wanted));
+        } else if constexpr (WORDS == 2 && VEC == 4) {
+            asm volatile("{ .reg .pred p; setp.ne.u32 p, %3, 0; mov.b32 %0, 0; mov.b32 %1, 0; @p ld.global.cs.v2.u32 {%0, %1}, [%2]; }"
+                         : "=&r"(w[0]), "=&r"(w[1]) : "l"(p), "r"((uint32_t)wanted));
+        } else if constexpr (VEC == 1) {
+            w[0] = 0;
+            if constexpr (sizeof(T) == 4)
+                asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; mov.b32 %0, 0; @p ld.global.cs.u32 %0, [%1]; }" : "=&r"(w[0]) : "l"(p), "r"((uint32_t)wanted));
+            else {
+                uint16_t h;
+                asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; mov.b16 %0, 0; @p ld.global.cs.u16 %0, [%1]; }" : "=&h"(h) : "l"(p), "r"((uint32_t)wanted));
+                w[0] = h;
+            }
+        } else {                                       // pairs off every boundary
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = 0;
+            if (wanted)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    if constexpr (sizeof(T) == 4) w[i] = __ldcs(reinterpret_cast<const unsigned int *>(p) + i);
+                    else w[i / 2] |= (uint32_t)__ldcs(reinterpret_cast<const unsigned short *>(p) + i) << (16 * (i & 1));
+                }
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[VEC]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) v[i] = __uint_as_float(w[i]);
+        } else if constexpr (VEC == 1) v[0] = low(w[0]);
+        else
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) { v[i] = low(w[i / 2]); v[i + 1] = high(w[i / 2]); }
+    }
+};
+
 inline bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 // Division of 64-bit task numbers by a launch constant: the upper half of a product with ceil(2^64 / d), exact while task * d < 2^64
