@@ -173,9 +173,12 @@ __global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_back
         if (c < hd) load_gain<VEC>(m.gain, c, gain[k]);
     }
     const int64_t rounds = (P.n + row_step - 1) / row_step;
+    int next = first < P.n ? __ldg(P.pos + first) : 0;     // the table waits for the position: asked for a round ahead
     for (int64_t t = 0; t < rounds; t++) {
         const int64_t row = first + t * row_step;
         const bool live = row < P.n;
+        const int at = min(max(next, 0), P.n_pos - 1);
+        next = row + row_step < P.n ? __ldg(P.pos + row + row_step) : 0;
         vec::Piece<T, VEC> x_piece[HEADS][NV];
         vec::Piece<D, VEC> d_piece[HEADS][NV];
         const T *at_x = reinterpret_cast<const T *>(m.x) + row * m.ld_x;
@@ -190,7 +193,6 @@ __global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_back
                 d_piece[u][k].fetch(at_d + h * hd + c, live && h < m.heads && c < hd);
             }
         }
-        const int at = live ? min(max(__ldg(P.pos + row), 0), P.n_pos - 1) : 0;
         float cs[NV][VEC / 2], sn[NV][VEC / 2];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
