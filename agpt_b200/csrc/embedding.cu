@@ -52,22 +52,19 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ emb, 
         id[u] = r < n ? token_of(ids, wide, r, vocab) : vocab;
     }
     for (int c = c0; c < d; c += lanes * VEC) {
-        float v[LOOK_ROWS][VEC];
+        vec::Piece<T, VEC> piece[LOOK_ROWS];
 #pragma unroll
-        for (int u = 0; u < LOOK_ROWS; u++) {
-            if (id[u] < vocab) vec::load<VEC>(emb + (int64_t)id[u] * ld + c, v[u]);
-            else
-#pragma unroll
-                for (int i = 0; i < VEC; i++) v[u][i] = 0.f;
-        }
+        for (int u = 0; u < LOOK_ROWS; u++) piece[u].fetch_kept(emb + (int64_t)id[u] * ld + c, id[u] < vocab);
 #pragma unroll
         for (int u = 0; u < LOOK_ROWS; u++) {
             const int64_t r = r0 + (int64_t)u * per_block;
             if (r >= n) break;
-            if (id[u] < vocab)
+            float v[VEC];
+            piece[u].values(v);
+            if (id[u] < vocab)                         // zero rows stay zero whatever the scale is
 #pragma unroll
-                for (int i = 0; i < VEC; i++) v[u][i] *= scale;
-            vec::store<VEC>(out + r * d + c, v[u]);
+                for (int i = 0; i < VEC; i++) v[i] *= scale;
+            vec::store<VEC>(out + r * d + c, v);
         }
     }
 }
@@ -75,7 +72,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ emb, 
 // ---- order of the rows by token: counting sort, least significant digit first -----------------------------------------------------
 // A pass counts the digits of each block's rows (count_kernel), turns the counts into places over the blocks (place_kernel) and moves
 // the pairs (move_kernel): a warp of a block owns a run of rows and has its own counters, so rows of one digit keep their order.
-constexpr int MOVE_WARPS = 8, DIGIT_BITS_MAX = 11;
+constexpr int MOVE_WARPS = 16, DIGIT_BITS_MAX = 11, PLACE_RUNS = 32;
 
 template <bool FIRST>
 __device__ __forceinline__ uint32_t key_of(const void *ids, int wide, const uint2 *in, int64_t i, uint32_t vocab) {
@@ -91,19 +88,19 @@ __global__ void __launch_bounds__(256) count_kernel(const void *__restrict__ ids
     for (int b = threadIdx.x; b < bins; b += 256) s_hist[b] = 0;
     __syncthreads();
     const int64_t i0 = (int64_t)blockIdx.x * chunk, i1 = min(i0 + chunk, n);
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) atomicAdd(&s_hist[(key_of<FIRST>(ids, wide, in, i, vocab) >> shift) & (bins - 1)], 1u);
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)blockIdx.x * bins + b] = s_hist[b];
 }
 
-// counts[block][digit] -> rows of the digit in earlier blocks; totals[digit].  A block has 32 digits and eight slices of the blocks.
-__global__ void __launch_bounds__(256) place_kernel(uint32_t *__restrict__ counts, int blocks, int bins, uint32_t *__restrict__ totals) {
+// counts[block][digit] -> rows of the digit in earlier blocks; totals[digit].  A block has 32 digits and PLACE_RUNS runs of the blocks.
+__global__ void __launch_bounds__(PLACE_RUNS * 32) place_kernel(uint32_t *__restrict__ counts, int blocks, int bins, uint32_t *__restrict__ totals) {
     pdl_wait();
     pdl_next();
-    __shared__ uint32_t s[8][32];
+    __shared__ uint32_t s[PLACE_RUNS][32];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
-    const int b0 = blocks * w / 8, b1 = blocks * (w + 1) / 8;
+    const int b0 = blocks * w / PLACE_RUNS, b1 = blocks * (w + 1) / PLACE_RUNS;
     uint32_t sum = 0;
     if (d < bins)
 #pragma unroll 8
@@ -113,12 +110,17 @@ __global__ void __launch_bounds__(256) place_kernel(uint32_t *__restrict__ count
     uint32_t at = 0;
     for (int k = 0; k < w; k++) at += s[k][lane];
     if (d >= bins) return;
-    if (w == 7) totals[d] = at + sum;
-#pragma unroll 8
-    for (int b = b0; b < b1; b++) {
-        const uint32_t x = counts[(int64_t)b * bins + d];
-        counts[(int64_t)b * bins + d] = at;
-        at += x;
+    if (w == PLACE_RUNS - 1) totals[d] = at + sum;
+    for (int first = b0; first < b1; first += 8) {
+        uint32_t x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = first + k < b1 ? counts[(int64_t)(first + k) * bins + d] : 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (first + k >= b1) break;
+            counts[(int64_t)(first + k) * bins + d] = at;
+            at += x[k];
+        }
     }
 }
 
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
     uint32_t *mine = s_at + w * bins, *start = s_at + MOVE_WARPS * bins;
     __shared__ uint32_t s_warp[MOVE_WARPS];
     for (int b = threadIdx.x; b < MOVE_WARPS * bins; b += MOVE_WARPS * 32) s_at[b] = 0;
-    // starts of the digits: a thread has bins / 256 neighbours (bins >= 256, or the threads behind have none)
+    // starts of the digits: a thread has neighbours, or none
     const int each = (bins + MOVE_WARPS * 32 - 1) / (MOVE_WARPS * 32);
     uint32_t sum = 0;
     for (int k = 0; k < each; k++) {
@@ -169,10 +171,15 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
         }
     }
     __syncthreads();
+    const auto load = [&](int64_t i) {
+        if (i >= i1) return make_uint2(0, 0);
+        return FIRST ? make_uint2(token_of(ids, wide, i, vocab), (uint32_t)i) : __ldg(in + i);
+    };
+    uint2 next = load(i0 + lane);
     for (int64_t i = i0; i < i1; i += 32) {
         const bool live = i + lane < i1;
-        uint2 p = make_uint2(0, 0);
-        if (live) p = FIRST ? make_uint2(token_of(ids, wide, i + lane, vocab), (uint32_t)(i + lane)) : __ldg(in + i + lane);
+        const uint2 p = next;
+        next = load(i + 32 + lane);
         const uint32_t digit = live ? (p.x >> shift) & (bins - 1) : 0xffffffffu;
         const uint32_t same = __match_any_sync(0xffffffffu, digit);
         uint32_t to = 0;
@@ -265,20 +272,19 @@ __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict
             const uint2 mine = p + lane < p1 ? __ldg(order + p + lane) : make_uint2(vocab, 0);
             const int live = (int)min((int64_t)32, p1 - p);
             for (int k0 = 0; k0 < live; k0 += U) {
-                float v[U][VEC];
+                vec::Piece<T, VEC> piece[U];
                 uint32_t key[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     key[u] = __shfl_sync(0xffffffffu, mine.x, k0 + u);
                     const uint32_t row = __shfl_sync(0xffffffffu, mine.y, k0 + u);
-                    if (k0 + u < live && key[u] < vocab && c < d) vec::load<VEC>(grad + (int64_t)row * ld + c, v[u]);
-                    else
-#pragma unroll
-                        for (int i = 0; i < VEC; i++) v[u][i] = 0.f;
+                    piece[u].fetch(grad + (int64_t)row * ld + c, k0 + u < live && key[u] < vocab && c < d);
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (k0 + u >= live) break;
+                    float v[VEC];
+                    piece[u].values(v);
                     if (key[u] != cur) {
                         if (begun_before) {
 #pragma unroll
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict
                         for (int i = 0; i < VEC; i++) acc[i] = 0.f;
                     }
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) acc[i] += v[u][i];
+                    for (int i = 0; i < VEC; i++) acc[i] += v[i];
                 }
             }
         }
@@ -330,47 +336,84 @@ __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict
     }
 }
 
-// Tokens that began in this block and go on behind it: tail, then the heads of the blocks that begin with the token.  The heads are cut into
-// as many runs as there are warps.
+// Tokens that began in a block of the sums and go on behind it: tail, then the heads of the blocks that begin with the token.  A warp has a block; where the heads
+// are many, all warps of the block come together and have a run of them each.
+constexpr int JOIN_ALONE = 16;
 template <typename O>
-__global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab, int64_t span, float scale, int accumulate,
+__global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab, int64_t span, int64_t blocks, float scale, int accumulate,
                                                     O *__restrict__ out, const float *__restrict__ head, const float *__restrict__ tail) {
     pdl_wait();
     pdl_next();
-    __shared__ float s_part[8][32];
-    __shared__ int64_t s_heads;
-    const int64_t p0 = (int64_t)blockIdx.x * span, p1 = p0 + span;         // the last block has nothing behind it and is not launched
-    const uint32_t key = __ldg(&order[p1 - 1].x);
-    if (key >= vocab || __ldg(&order[p1].x) != key) return;
-    if (p0 > 0 && __ldg(&order[p0].x) == key && __ldg(&order[p0 - 1].x) == key) return;      // began before
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    if (w == 0) {
-        int64_t heads = 1;
-        for (bool more = true; more; ) {
-            const int64_t p = p1 + (heads + lane) * span;
-            const uint32_t b = __ballot_sync(0xffffffffu, p < n && __ldg(&order[p].x) == key);
-            heads += b == 0xffffffffu ? 32 : __ffs(~b) - 1;
-            more = b == 0xffffffffu;
-        }
-        if (lane == 0) s_heads = heads;
-    }
-    __syncthreads();
-    const int64_t heads = s_heads, h0 = heads * w / 8, h1 = heads * (w + 1) / 8;
-    for (int c0 = blockIdx.y * 32; c0 < d; c0 += gridDim.y * 32) {
-        const int c = c0 + lane;
-        float acc = 0.f;
-        if (c < d) {
-            if (w == 0) acc = tail[(int64_t)blockIdx.x * d + c];
+    __shared__ float s_part[8][128];
+    __shared__ int64_t s_heads[8];
+    __shared__ uint32_t s_key[8];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c0 = blockIdx.y * 128;
+    const bool whole = (d & 3) == 0;
+    // sums of heads [h0, h1) behind block b, and of its tail; four columns a lane, neighbours if they lie on 16-byte boundaries
+    const auto column = [&](int i) { return c0 + (whole ? lane * 4 + i : lane + 32 * i); };
+    const auto add = [&](int64_t b, int64_t h0, int64_t h1, bool with_tail, float (&acc)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = with_tail && column(i) < d ? tail[b * d + column(i)] : 0.f;
+        if (whole) {
+            if (column(0) < d)
 #pragma unroll 8
-            for (int64_t h = h0; h < h1; h++) acc += head[(blockIdx.x + 1 + h) * d + c];
+                for (int64_t h = h0; h < h1; h++) {
+                    const float4 v = __ldcs(reinterpret_cast<const float4 *>(head + (b + 1 + h) * d + column(0)));
+                    acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
+                }
+        } else {
+#pragma unroll 2
+            for (int64_t h = h0; h < h1; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (column(i) < d) acc[i] += __ldcs(head + (b + 1 + h) * d + column(i));
         }
-        s_part[w][lane] = acc;
+    };
+    const int64_t b = (int64_t)blockIdx.x * 8 + w, p0 = b * span, p1 = p0 + span;
+    int64_t heads = 0;
+    uint32_t key = vocab;
+    if (b < blocks && p1 < n) {
+        key = __ldg(&order[p1 - 1].x);
+        const bool goes_on = key < vocab && __ldg(&order[p1].x) == key;
+        const bool before = p0 > 0 && __ldg(&order[p0].x) == key && __ldg(&order[p0 - 1].x) == key;
+        if (goes_on && !before) {
+            heads = 1;
+            for (bool more = true; more; ) {
+                const int64_t p = p1 + (heads + lane) * span;
+                const uint32_t bits = __ballot_sync(0xffffffffu, p < n && __ldg(&order[p].x) == key);
+                heads += bits == 0xffffffffu ? 32 : __ffs(~bits) - 1;
+                more = bits == 0xffffffffu;
+            }
+        }
+    }
+    if (heads && heads <= JOIN_ALONE) {
+        float acc[4];
+        add(b, 0, heads, true, acc);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (column(i) < d) {
+                float one[1] = {acc[i]};
+                write_row<O, 1>(out, (int64_t)key * d + column(i), one, scale, accumulate);
+            }
+    }
+    if (lane == 0) { s_heads[w] = heads; s_key[w] = key; }
+    __syncthreads();
+    for (int k = 0; k < 8; k++) {
+        const int64_t many = s_heads[k];
+        if (many <= JOIN_ALONE) continue;
+        float acc[4];
+        add((int64_t)blockIdx.x * 8 + k, many * w / 8, many * (w + 1) / 8, w == 0, acc);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s_part[w][lane + 32 * i] = acc[i];
         __syncthreads();
-        if (w == 0 && c < d) {
-            for (int k = 1; k < 8; k++) acc += s_part[k][lane];
-            float one[1] = {acc};
-            write_row<O, 1>(out, (int64_t)key * d + c, one, scale, accumulate);
-        }
+        if (w == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (column(i) < d) {
+                    float one[1] = {0.f};
+                    for (int x = 0; x < 8; x++) one[0] += s_part[x][lane + 32 * i];
+                    write_row<O, 1>(out, (int64_t)s_key[k] * d + column(i), one, scale, accumulate);
+                }
         __syncthreads();
     }
 }
@@ -462,7 +505,7 @@ Sizes sizes_of(int64_t n, int d, int64_t vocab) {
     z.bits = (bits + z.passes - 1) / z.passes;
     const int64_t sms = vec::sm_count();
     z.chunk = (n + 2 * sms - 1) / (2 * sms);
-    z.chunk = z.chunk < 1024 ? 1024 : (z.chunk + 255) / 256 * 256;
+    z.chunk = z.chunk < 1024 ? 1024 : (z.chunk + 32 * MOVE_WARPS - 1) / (32 * MOVE_WARPS) * (32 * MOVE_WARPS);
     z.chunks = (n + z.chunk - 1) / z.chunk;
     z.run = 64;
     while (z.run > 8 && (n + SUM_WARPS * z.run - 1) / (SUM_WARPS * z.run) * ((d + 127) / 128) < 8 * sms) z.run /= 2;
@@ -491,7 +534,7 @@ int sort_pass(const void *ids, int wide, const uint2 *in, int64_t n, const Sizes
         if (dev >= 0 && dev < 64) set[dev] = true;
     }
     pdl_launch(count_kernel<FIRST>, (unsigned)z.chunks, 256, (size_t)bins * 4, st, ids, wide, in, n, z.chunk, vocab, shift, bins, counts);
-    pdl_launch(place_kernel, (unsigned)((bins + 31) / 32), 256, 0, st, counts, (int)z.chunks, bins, totals);
+    pdl_launch(place_kernel, (unsigned)((bins + 31) / 32), PLACE_RUNS * 32, 0, st, counts, (int)z.chunks, bins, totals);
     pdl_launch(move_kernel<FIRST>, (unsigned)z.chunks, MOVE_WARPS * 32, smem, st, ids, wide, in, n, z.chunk, vocab, shift, z.bits, (const uint32_t *)counts,
                (const uint32_t *)totals, out);
     return AGPT_OK;
@@ -515,7 +558,8 @@ int grad_sorted(const T *grad, int64_t ld, const void *ids, int wide, O *out, in
     pdl_launch(sum_kernel<T, O, VEC>, dim3((unsigned)(z.blocks + fill), slices), SUM_WARPS * 32, 0, st, grad, ld, order, n, d, vocab, z.run, z.blocks, scale, accumulate,
                out, head, tail);
     if (z.blocks > 1)
-        pdl_launch(join_kernel<O>, dim3((unsigned)(z.blocks - 1), (unsigned)((d + 31) / 32)), 256, 0, st, order, n, d, vocab, (int64_t)SUM_WARPS * z.run, scale, accumulate,
+        pdl_launch(join_kernel<O>, dim3((unsigned)((z.blocks + 7) / 8), (unsigned)((d + 127) / 128)), 256, 0, st, order, n, d, vocab, (int64_t)SUM_WARPS * z.run, z.blocks, scale,
+                   accumulate,
                    out, (const float *)head, (const float *)tail);
     return launch_status("embedding_grad_sorted");
 }

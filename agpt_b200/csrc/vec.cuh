@@ -94,6 +94,21 @@ template <typename T, int VEC> struct Piece {
                 }
         }
     }
+    // the same through the caches, for rows that are read again
+    __device__ __forceinline__ void fetch_kept(const T *p, bool wanted) {
+        if constexpr (WORDS >= 4) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4)
+                asm volatile("{ .reg .pred p; setp.ne.u32 p, %5, 0; mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0; @p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4]; }"
+                             : "=&r"(w[i]), "=&r"(w[i + 1]), "=&r"(w[i + 2]), "=&r"(w[i + 3]) : "l"(reinterpret_cast<const uint32_t *>(p) + i), "r"((uint32_t)wanted));
+        } else if constexpr (sizeof(T) == 4) {
+            asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; mov.b32 %0, 0; @p ld.global.nc.u32 %0, [%1]; }" : "=&r"(w[0]) : "l"(p), "r"((uint32_t)wanted));
+        } else {
+            uint16_t h;
+            asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; mov.b16 %0, 0; @p ld.global.nc.u16 %0, [%1]; }" : "=&h"(h) : "l"(p), "r"((uint32_t)wanted));
+            w[0] = h;
+        }
+    }
     __device__ __forceinline__ void values(float (&v)[VEC]) const {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
