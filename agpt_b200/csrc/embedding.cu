@@ -9,6 +9,9 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "../../include/agpt_b200.h"
 #include "internal.h"
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
 // A warp has `run` places of the order and 32 * VEC columns, a block SUM_WARPS warps side by side.  Tokens that end where they began are
 // written; the warps' first and last sums meet in shared memory; what a block has of a token that began before it goes to head[block], of
 // one that goes on behind it to tail[block], and join_kernel adds tail and heads in order.
-constexpr int SUM_WARPS = 8, FILL_TOKENS = 64;
+constexpr int SUM_WARPS = 8, SUM_RING = 8, FILL_TOKENS = 64;
 
 template <typename O, int VEC>
 __device__ __forceinline__ void write_row(O *out, int64_t at, float (&v)[VEC], float scale, int accumulate) {
@@ -245,12 +248,13 @@ __device__ void fill_absent(const uint2 *order, int64_t n, O *out, int d, uint32
 }
 
 template <typename T, typename O, int VEC>
-__global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict__ grad, int64_t ld, const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab,
+__global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restrict__ grad, int64_t ld, const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab,
                                                               int run, int64_t blocks, float scale, int accumulate, O *__restrict__ out, float *__restrict__ head,
                                                               float *__restrict__ tail) {
     pdl_wait();
     pdl_next();
-    constexpr int COLS = 32 * VEC, U = 8;
+    constexpr int COLS = 32 * VEC;
+    extern __shared__ __align__(16) unsigned char s_rows[];     // VEC > 1: [SUM_WARPS][SUM_RING] rows of 512 bytes
     __shared__ float s_part[SUM_WARPS][2][COLS];
     __shared__ uint32_t s_first[SUM_WARPS], s_last[SUM_WARPS];
     __shared__ uint8_t s_in[SUM_WARPS], s_out[SUM_WARPS], s_through[SUM_WARPS];
@@ -261,6 +265,8 @@ __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * COLS + lane * VEC;
     const int64_t p0 = ((int64_t)blockIdx.x * SUM_WARPS + w) * run, p1 = min(p0 + run, n);
     if (p0 < n) {
+        const uint2 none = make_uint2(vocab, 0);
+        const uint2 near = p0 + lane < p1 ? __ldg(order + p0 + lane) : none, far = p0 + 32 + lane < p1 ? __ldg(order + p0 + 32 + lane) : none;      // at most 64 places
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; i++) acc[i] = 0.f;
@@ -268,35 +274,64 @@ __global__ void __launch_bounds__(SUM_WARPS * 32) sum_kernel(const T *__restrict
         const bool in = p0 > 0 && __ldg(&order[p0 - 1].x) == first, goes_on = p1 < n && __ldg(&order[p1].x) == last;
         uint32_t cur = first;
         bool begun_before = in;
-        for (int64_t p = p0; p < p1; p += 32) {
-            const uint2 mine = p + lane < p1 ? __ldg(order + p + lane) : make_uint2(vocab, 0);
-            const int live = (int)min((int64_t)32, p1 - p);
+        const int live = (int)(p1 - p0);
+        const auto pair = [&](int k) {
+            const uint2 x = k < 32 ? near : far;
+            return make_uint2(__shfl_sync(0xffffffffu, x.x, k & 31), __shfl_sync(0xffffffffu, x.y, k & 31));
+        };
+        const auto add = [&](uint32_t key, const float (&v)[VEC]) {
+            if (key != cur) {
+                if (begun_before) {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) s_part[w][0][lane * VEC + i] = acc[i];
+                } else if (cur < vocab && c < d) write_row<O, VEC>(out, (int64_t)cur * d + c, acc, scale, accumulate);
+                cur = key;
+                begun_before = false;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) acc[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; i++) acc[i] += v[i];
+        };
+        if constexpr (VEC > 1) {
+            // Rows come by asynchronous copies into a ring that only the copying lane reads: SUM_RING rows of every warp are on their way without a register each.
+            // (Eight rows in registers at a time left the loads waiting for the sums: 142 us at 1.4M x 128, two batches of four 150 to 175, this 119.)
+            const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_rows) + (w * SUM_RING * 32 + lane) * 16;
+            const auto fetch = [&](int k) {
+                if (k < live) {
+                    const uint2 x = pair(k);
+                    if (x.x < vocab && c < d)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (k % SUM_RING) * 512), "l"(grad + (int64_t)x.y * ld + c) : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll
+            for (int k = 0; k < SUM_RING - 1; k++) fetch(k);
+            for (int k = 0; k < live; k++) {
+                fetch(k + SUM_RING - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(SUM_RING - 1) : "memory");
+                vec::Piece<T, VEC> piece;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(piece.w[0]), "=r"(piece.w[1]), "=r"(piece.w[2]), "=r"(piece.w[3]) : "r"(ring + (k % SUM_RING) * 512) : "memory");
+                float v[VEC];
+                piece.values(v);
+                add(pair(k).x, v);
+            }
+        } else {
+            constexpr int U = 8;
             for (int k0 = 0; k0 < live; k0 += U) {
                 vec::Piece<T, VEC> piece[U];
-                uint32_t key[U];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    key[u] = __shfl_sync(0xffffffffu, mine.x, k0 + u);
-                    const uint32_t row = __shfl_sync(0xffffffffu, mine.y, k0 + u);
-                    piece[u].fetch(grad + (int64_t)row * ld + c, k0 + u < live && key[u] < vocab && c < d);
+                    const uint2 x = pair(k0 + u);
+                    piece[u].fetch(grad + (int64_t)x.y * ld + c, k0 + u < live && x.x < vocab && c < d);
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
+                    const uint32_t key = pair(k0 + u).x;
                     if (k0 + u >= live) break;
                     float v[VEC];
                     piece[u].values(v);
-                    if (key[u] != cur) {
-                        if (begun_before) {
-#pragma unroll
-                            for (int i = 0; i < VEC; i++) s_part[w][0][lane * VEC + i] = acc[i];
-                        } else if (cur < vocab && c < d) write_row<O, VEC>(out, (int64_t)cur * d + c, acc, scale, accumulate);
-                        cur = key[u];
-                        begun_before = false;
-#pragma unroll
-                        for (int i = 0; i < VEC; i++) acc[i] = 0.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) acc[i] += v[i];
+                    add(key, v);
                 }
             }
         }
@@ -520,19 +555,27 @@ Sizes sizes_of(int64_t n, int d, int64_t vocab) {
     return z;
 }
 
+// dynamic shared memory beyond 48 KB, allowed once per kernel and device
+template <typename... P>
+int allow_smem(void (*kernel)(P...), int bytes) {
+    static std::mutex lock;
+    static std::set<std::pair<const void *, int>> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> hold(lock);
+    if (done.count({(const void *)kernel, dev})) return AGPT_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "embedding_grad_sorted: %s", cudaGetErrorString(e));
+    done.insert({(const void *)kernel, dev});
+    return AGPT_OK;
+}
+
 template <bool FIRST>
 int sort_pass(const void *ids, int wide, const uint2 *in, int64_t n, const Sizes &z, uint32_t vocab, int pass, char *ws, uint2 *out, cudaStream_t st) {
     const int bins = 1 << z.bits, shift = pass * z.bits;
     uint32_t *counts = (uint32_t *)(ws + z.at_counts), *totals = (uint32_t *)(ws + z.at_totals);
     const size_t smem = (size_t)(MOVE_WARPS + 1) * bins * 4;
-    static bool set[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(move_kernel<FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (MOVE_WARPS + 1) * 4 << DIGIT_BITS_MAX);
-        if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "embedding_grad_sorted: %s", cudaGetErrorString(e));
-        if (dev >= 0 && dev < 64) set[dev] = true;
-    }
+    if (int rc = allow_smem(move_kernel<FIRST>, (MOVE_WARPS + 1) * 4 << DIGIT_BITS_MAX)) return rc;
     pdl_launch(count_kernel<FIRST>, (unsigned)z.chunks, 256, (size_t)bins * 4, st, ids, wide, in, n, z.chunk, vocab, shift, bins, counts);
     pdl_launch(place_kernel, (unsigned)((bins + 31) / 32), PLACE_RUNS * 32, 0, st, counts, (int)z.chunks, bins, totals);
     pdl_launch(move_kernel<FIRST>, (unsigned)z.chunks, MOVE_WARPS * 32, smem, st, ids, wide, in, n, z.chunk, vocab, shift, z.bits, (const uint32_t *)counts,
@@ -555,7 +598,9 @@ int grad_sorted(const T *grad, int64_t ld, const void *ids, int wide, O *out, in
         if (int rc = sort_pass<false>(nullptr, 0, pairs[(p - 1) & 1], n, z, vocab, p, ws, pairs[p & 1], st)) return rc;
     const uint2 *order = pairs[(z.passes - 1) & 1];
     float *head = (float *)(ws + z.at_head), *tail = (float *)(ws + z.at_tail);
-    pdl_launch(sum_kernel<T, O, VEC>, dim3((unsigned)(z.blocks + fill), slices), SUM_WARPS * 32, 0, st, grad, ld, order, n, d, vocab, z.run, z.blocks, scale, accumulate,
+    if (VEC > 1)
+        if (int rc = allow_smem(sum_kernel<T, O, VEC>, SUM_WARPS * SUM_RING * 512)) return rc;
+    pdl_launch(sum_kernel<T, O, VEC>, dim3((unsigned)(z.blocks + fill), slices), SUM_WARPS * 32, VEC > 1 ? SUM_WARPS * SUM_RING * 512 : 0, st, grad, ld, order, n, d, vocab, z.run, z.blocks, scale, accumulate,
                out, head, tail);
     if (z.blocks > 1)
         pdl_launch(join_kernel<O>, dim3((unsigned)((z.blocks + 7) / 8), (unsigned)((d + 127) / 128)), 256, 0, st, order, n, d, vocab, (int64_t)SUM_WARPS * z.run, z.blocks, scale,
@@ -616,7 +661,7 @@ extern "C" int64_t agpt_b200_embedding_grad_sorted_workspace_bytes(int64_t n, in
 }
 
 extern "C" int agpt_b200_embedding_grad_sorted(const void *d_grad, int64_t grad_ld, int type, const void *d_ids, int ids64, void *d_emb_grad, int out_type, int64_t n,
-                                               int d_model, int vocab, float scale, int accumulate, void *d_workspace, int64_t workspace_bytes, void *stream) {
+                                               int d_model, int vocab, float scale, int accumulate, void *d_workspace, int64_t workspace_bytes, void *stream) try {
     if (int rc = check_sizes("embedding_grad_sorted", n, d_model, grad_ld, vocab, type)) return rc;
     if (out_type != AGPT_KV_F32 && out_type != AGPT_KV_BF16) return agpt_set_error(AGPT_E_ARG, "embedding_grad_sorted: the table's gradient is float32 (0) or bfloat16 (1)");
     if (!d_emb_grad || (n && (!d_grad || !d_ids))) return agpt_set_error(AGPT_E_ARG, "embedding_grad_sorted: bad argument");
@@ -627,4 +672,4 @@ extern "C" int agpt_b200_embedding_grad_sorted(const void *d_grad, int64_t grad_
     if (type == AGPT_KV_BF16)
         return grad_by_output((const bf16 *)d_grad, grad_ld, d_ids, ids64, d_emb_grad, out_type, n, d_model, (uint32_t)vocab, scale, accumulate, (char *)d_workspace, st);
     return grad_by_output((const float *)d_grad, grad_ld, d_ids, ids64, d_emb_grad, out_type, n, d_model, (uint32_t)vocab, scale, accumulate, (char *)d_workspace, st);
-}
+} AGPT_CATCH("embedding_grad_sorted")
