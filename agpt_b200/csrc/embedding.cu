@@ -77,22 +77,35 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ emb, 
 // the pairs (move_kernel): a warp of a block owns a run of rows and has its own counters, so rows of one digit keep their order.
 constexpr int MOVE_WARPS = 16, DIGIT_BITS_MAX = 11, PLACE_RUNS = 32;
 
-template <bool FIRST>
-__device__ __forceinline__ uint32_t key_of(const void *ids, int wide, const uint2 *in, int64_t i, uint32_t vocab) {
-    return FIRST ? token_of(ids, wide, i, vocab) : __ldg(&in[i].x);
+// What a pass reads: the caller's tokens, int32 or int64, or the pairs of the pass before.  Known to the compiler, and loads are made without a branch around
+// them (behind the last row the last one again): a loop of guarded loads waits for each in turn (the counts of 1.4M rows took 13 us).
+enum { IDS32, IDS64, PAIRS };
+template <int SOURCE> __device__ __forceinline__ uint32_t key_at(const void *source, int64_t i, uint32_t vocab) {
+    if constexpr (SOURCE == PAIRS) return __ldg(&reinterpret_cast<const uint2 *>(source)[i].x);
+    else return token_of(source, SOURCE == IDS64, i, vocab);
+}
+template <int SOURCE> __device__ __forceinline__ uint2 pair_at(const void *source, int64_t i, uint32_t vocab) {
+    if constexpr (SOURCE == PAIRS) return __ldg(reinterpret_cast<const uint2 *>(source) + i);
+    else return make_uint2(token_of(source, SOURCE == IDS64, i, vocab), (uint32_t)i);
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(256) count_kernel(const void *__restrict__ ids, int wide, const uint2 *__restrict__ in, int64_t n, int64_t chunk, uint32_t vocab,
-                                                     int shift, int bins, uint32_t *__restrict__ counts) {
+template <int SOURCE>
+__global__ void __launch_bounds__(256) count_kernel(const void *__restrict__ source, int64_t n, int64_t chunk, uint32_t vocab, int shift, int bins,
+                                                     uint32_t *__restrict__ counts) {
     pdl_wait();
     pdl_next();
     extern __shared__ uint32_t s_hist[];
     for (int b = threadIdx.x; b < bins; b += 256) s_hist[b] = 0;
     __syncthreads();
     const int64_t i0 = (int64_t)blockIdx.x * chunk, i1 = min(i0 + chunk, n);
-#pragma unroll 8
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) atomicAdd(&s_hist[(key_of<FIRST>(ids, wide, in, i, vocab) >> shift) & (bins - 1)], 1u);
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256 * 8) {
+        uint32_t key[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) key[k] = key_at<SOURCE>(source, min(i + 256 * k, i1 - 1), vocab);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + 256 * k < i1) atomicAdd(&s_hist[(key[k] >> shift) & (bins - 1)], 1u);
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += 256) counts[(int64_t)blockIdx.x * bins + b] = s_hist[b];
 }
@@ -127,9 +140,8 @@ __global__ void __launch_bounds__(PLACE_RUNS * 32) place_kernel(uint32_t *__rest
     }
 }
 
-template <bool FIRST>
-__global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__restrict__ ids, int wide, const uint2 *__restrict__ in, int64_t n, int64_t chunk,
-                                                                uint32_t vocab, int shift, int bits, const uint32_t *__restrict__ counts,
+template <int SOURCE>
+__global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__restrict__ source, int64_t n, int64_t chunk, uint32_t vocab, int shift, int bits, const uint32_t *__restrict__ counts,
                                                                 const uint32_t *__restrict__ totals, uint2 *__restrict__ out) {
     pdl_wait();
     pdl_next();
@@ -161,8 +173,14 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
     }
     // digits of each warp's rows
     const int64_t own = chunk / MOVE_WARPS, i0 = (int64_t)blockIdx.x * chunk + w * own, i1 = min(i0 + own, n);
-#pragma unroll 4
-    for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[(key_of<FIRST>(ids, wide, in, i, vocab) >> shift) & (bins - 1)], 1u);
+    for (int64_t i = i0 + lane; i < i1; i += 32 * 8) {
+        uint32_t key[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) key[k] = key_at<SOURCE>(source, min(i + 32 * k, i1 - 1), vocab);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + 32 * k < i1) atomicAdd(&mine[(key[k] >> shift) & (bins - 1)], 1u);
+    }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += MOVE_WARPS * 32) {
         uint32_t t = start[b] + __ldg(counts + (int64_t)blockIdx.x * bins + b);
@@ -174,10 +192,8 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
         }
     }
     __syncthreads();
-    const auto load = [&](int64_t i) {
-        if (i >= i1) return make_uint2(0, 0);
-        return FIRST ? make_uint2(token_of(ids, wide, i, vocab), (uint32_t)i) : __ldg(in + i);
-    };
+    if (i0 >= i1) return;
+    const auto load = [&](int64_t i) { return pair_at<SOURCE>(source, min(i, i1 - 1), vocab); };
     uint2 next = load(i0 + lane);
     for (int64_t i = i0; i < i1; i += 32) {
         const bool live = i + lane < i1;
@@ -412,13 +428,16 @@ __global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ ord
         const bool goes_on = key < vocab && __ldg(&order[p1].x) == key;
         const bool before = p0 > 0 && __ldg(&order[p0].x) == key && __ldg(&order[p0 - 1].x) == key;
         if (goes_on && !before) {
-            heads = 1;
-            for (bool more = true; more; ) {
-                const int64_t p = p1 + (heads + lane) * span;
-                const uint32_t bits = __ballot_sync(0xffffffffu, p < n && __ldg(&order[p].x) == key);
-                heads += bits == 0xffffffffu ? 32 : __ffs(~bits) - 1;
-                more = bits == 0xffffffffu;
+            // blocks behind that begin with the token: they are the first ones, so 32 are asked at a time, near ones first, then by 32nds of what is left
+            int64_t low = 1, high = blocks - b;                        // `low` of them are known to, from `high` on none does
+            for (int64_t step = 1; low < high; step = (high - low + 31) / 32) {
+                const int64_t h = low + lane * step, p = p1 + h * span;
+                const int yes = __popc(__ballot_sync(0xffffffffu, h < high && p < n && __ldg(&order[p].x) == key));
+                if (yes < 32) high = min(high, low + yes * step);
+                low = yes ? low + (yes - 1) * step + 1 : low;
+                if (yes == 0) break;
             }
+            heads = low;
         }
     }
     if (heads && heads <= JOIN_ALONE) {
@@ -570,15 +589,15 @@ int allow_smem(void (*kernel)(P...), int bytes) {
     return AGPT_OK;
 }
 
-template <bool FIRST>
-int sort_pass(const void *ids, int wide, const uint2 *in, int64_t n, const Sizes &z, uint32_t vocab, int pass, char *ws, uint2 *out, cudaStream_t st) {
+template <int SOURCE>
+int sort_pass(const void *source, int64_t n, const Sizes &z, uint32_t vocab, int pass, char *ws, uint2 *out, cudaStream_t st) {
     const int bins = 1 << z.bits, shift = pass * z.bits;
     uint32_t *counts = (uint32_t *)(ws + z.at_counts), *totals = (uint32_t *)(ws + z.at_totals);
     const size_t smem = (size_t)(MOVE_WARPS + 1) * bins * 4;
-    if (int rc = allow_smem(move_kernel<FIRST>, (MOVE_WARPS + 1) * 4 << DIGIT_BITS_MAX)) return rc;
-    pdl_launch(count_kernel<FIRST>, (unsigned)z.chunks, 256, (size_t)bins * 4, st, ids, wide, in, n, z.chunk, vocab, shift, bins, counts);
+    if (int rc = allow_smem(move_kernel<SOURCE>, (MOVE_WARPS + 1) * 4 << DIGIT_BITS_MAX)) return rc;
+    pdl_launch(count_kernel<SOURCE>, (unsigned)z.chunks, 256, (size_t)bins * 4, st, source, n, z.chunk, vocab, shift, bins, counts);
     pdl_launch(place_kernel, (unsigned)((bins + 31) / 32), PLACE_RUNS * 32, 0, st, counts, (int)z.chunks, bins, totals);
-    pdl_launch(move_kernel<FIRST>, (unsigned)z.chunks, MOVE_WARPS * 32, smem, st, ids, wide, in, n, z.chunk, vocab, shift, z.bits, (const uint32_t *)counts,
+    pdl_launch(move_kernel<SOURCE>, (unsigned)z.chunks, MOVE_WARPS * 32, smem, st, source, n, z.chunk, vocab, shift, z.bits, (const uint32_t *)counts,
                (const uint32_t *)totals, out);
     return AGPT_OK;
 }
@@ -593,9 +612,9 @@ int grad_sorted(const T *grad, int64_t ld, const void *ids, int wide, O *out, in
     }
     const Sizes z = sizes_of(n, d, vocab);
     uint2 *pairs[2] = {(uint2 *)(ws + z.at_pairs), (uint2 *)(ws + z.at_pairs) + n};
-    if (int rc = sort_pass<true>(ids, wide, nullptr, n, z, vocab, 0, ws, pairs[0], st)) return rc;
+    if (int rc = wide ? sort_pass<IDS64>(ids, n, z, vocab, 0, ws, pairs[0], st) : sort_pass<IDS32>(ids, n, z, vocab, 0, ws, pairs[0], st)) return rc;
     for (int p = 1; p < z.passes; p++)
-        if (int rc = sort_pass<false>(nullptr, 0, pairs[(p - 1) & 1], n, z, vocab, p, ws, pairs[p & 1], st)) return rc;
+        if (int rc = sort_pass<PAIRS>(pairs[(p - 1) & 1], n, z, vocab, p, ws, pairs[p & 1], st)) return rc;
     const uint2 *order = pairs[(z.passes - 1) & 1];
     float *head = (float *)(ws + z.at_head), *tail = (float *)(ws + z.at_tail);
     if (VEC > 1)
