@@ -32,6 +32,12 @@ __device__ __forceinline__ float2 values2(uint32_t c) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
+// the larger of two magnitudes (with some sign), NaN if one of them is
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+    float r;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // what a scale byte stands for
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s == 255 ? 0x7fc00000u : s ? s << 23 : 0x00400000u); }
 
@@ -65,11 +71,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ x, int6
     uint32_t s4 = 0;
 #pragma unroll
     for (int u = 0; u < PACK_ROWS; u++) {
-        uint32_t top = 0;                              // magnitudes in order of their bits, infinity and NaN above all
+        float most = 0.f;                              // NaN where there is one
 #pragma unroll
-        for (int i = 0; i < VEC; i++) top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
+        for (int i = 0; i < VEC; i++) most = max_magnitude(most, v[u][i]);
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(group, top, o));
+        for (int o = LANES / 2; o > 0; o >>= 1) most = max_magnitude(most, __shfl_xor_sync(group, most, o));
+        const uint32_t top = __float_as_uint(most) & 0x7fffffffu;
         // 2^k <= top < 2^(k+1), k = (top >> 23) - 127: top <= 448 * 2^(k-8) = 1.75 * 2^k, or one more
         const int e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), -110);
         const bool bad = top >= 0x7f800000u;
@@ -79,9 +86,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ x, int6
 #pragma unroll
         for (int i = 0; i < VEC; i += 4) {
             uint32_t w = codes2(v[u][i] * down, v[u][i + 1] * down) | codes2(v[u][i + 2] * down, v[u][i + 3] * down) << 16;
+            // a byte of magnitude 0 (bit 7 of the sum stays clear) whose value is not: the smallest code
+            uint32_t some = 0;
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (v[u][i + k] != 0.f && !(w >> (8 * k) & 0x7f)) w |= 1u << (8 * k) | (v[u][i + k] < 0.f ? 0x80u << (8 * k) : 0u);
+            for (int k = 0; k < 4; k++) some |= v[u][i + k] != 0.f ? 1u << (8 * k) : 0;
+            w |= ~(((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) >> 7) & some;
             // 256 * 2^120 and above are no float32: what rounds there takes 240 * 2^120
             if (e == 120)
 #pragma unroll
@@ -91,8 +100,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ x, int6
         }
         if (r0 + u < n) {
             uint8_t *to = codes + (r0 + u) * (int64_t)blocks * 32 + c;
-            if (VEC == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(word[0], word[VEC / 4 - 1]);
-            else *reinterpret_cast<uint32_t *>(to) = word[0];
+            if (VEC == 8) __stcs(reinterpret_cast<uint2 *>(to), make_uint2(word[0], word[VEC / 4 - 1]));
+            else __stcs(reinterpret_cast<uint32_t *>(to), word[0]);
         }
     }
     // rows behind the last lie inside the pitch, which is a multiple of 16
@@ -121,7 +130,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t *__restrict__
         float v[4] = {a.x * f, a.y * f, d.x * f, d.y * f};
         float *to = out + (r0 + u) * cols + c;
         if (WHOLE) {
-            if (c < cols) vec::store<4>(to, v);
+            if (c < cols) vec::store_past<4>(to, v);
         } else
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
         }
         float *to = out + (r0 + u) * cols + c;
         if (WHOLE) {
-            if (c < cols) vec::store<4>(to, v[u]);
+            if (c < cols) vec::store_past<4>(to, v[u]);
         } else
 #pragma unroll
             for (int i = 0; i < 4; i++)

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ emb, 
             if (id[u] < vocab)                         // zero rows stay zero whatever the scale is
 #pragma unroll
                 for (int i = 0; i < VEC; i++) v[i] *= scale;
-            vec::store<VEC>(out + r * d + c, v);
+            vec::store_past<VEC>(out + r * d + c, v);
         }
     }
 }
@@ -230,7 +230,7 @@ __device__ __forceinline__ void write_row(O *out, int64_t at, float (&v)[VEC], f
 #pragma unroll
         for (int i = 0; i < VEC; i++) v[i] *= scale;
     }
-    vec::store<VEC>(out + at, v);
+    vec::store_past<VEC>(out + at, v);
 }
 
 // zero rows of the tokens that no row has

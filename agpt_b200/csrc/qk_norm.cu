@@ -51,8 +51,8 @@ template <int LOG2> __device__ __forceinline__ float group_sum(float v, int lane
     return v;
 }
 template <int VEC> __device__ __forceinline__ void store_either(void *p, int64_t at, int wide, const float (&v)[VEC]) {
-    if (wide) vec::store<VEC>(reinterpret_cast<float *>(p) + at, v);
-    else vec::store<VEC>(reinterpret_cast<bf16 *>(p) + at, v);
+    if (wide) vec::store_past<VEC>(reinterpret_cast<float *>(p) + at, v);
+    else vec::store_past<VEC>(reinterpret_cast<bf16 *>(p) + at, v);
 }
 // VEC entries of a table or a gain, by 16 bytes where the rows allow it
 template <int VEC> __device__ __forceinline__ void load_cached(const float *p, float (&v)[VEC]) {

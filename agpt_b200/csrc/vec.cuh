@@ -122,6 +122,18 @@ template <typename T, int VEC> struct Piece {
 
 inline bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
+// outputs larger than the caches: written past them
+template <int VEC> __device__ __forceinline__ void store_past(float *p, const float (&v)[VEC]) {
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) __stcs(reinterpret_cast<float4 *>(p) + i / 4, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+    } else store<VEC>(p, v);
+}
+template <int VEC> __device__ __forceinline__ void store_past(__nv_bfloat16 *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 8) __stcs(reinterpret_cast<uint4 *>(p), make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])));
+    else store<VEC>(p, v);
+}
+
 // Division of 64-bit task numbers by a launch constant: the upper half of a product with ceil(2^64 / d), exact while task * d < 2^64
 struct Divide {
     uint64_t m;
