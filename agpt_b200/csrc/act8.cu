@@ -41,39 +41,44 @@ __device__ __forceinline__ float max_magnitude(float a, float b) {
 // what a scale byte stands for
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s == 255 ? 0x7fc00000u : s ? s << 23 : 0x00400000u); }
 
-// A group of 32 / VEC lanes has a block of PACK_ROWS consecutive rows: their loads are in flight together and their scale bytes are neighbours.
+// A group of lanes has a block of PACK_ROWS consecutive rows: their loads are in flight together and their scale bytes are neighbours.  A lane has PIECES pieces of
+// VEC columns, eight values where rows allow it: what a block costs once (its maximum across lanes, its exponent) is the larger part of the arithmetic, and that
+// is what bounds the kernel (four values a lane: 276 us at 560k x 512, ALU pipe at 77 %).
 constexpr int PACK_ROWS = 4;
-template <typename T, int VEC, bool WHOLE>
+template <typename T, int VEC, int PIECES, bool WHOLE>
 __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ x, int64_t ld, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, int64_t n, int cols,
                                                     int blocks, int64_t pitch, vec::Divide by_blocks, int64_t tasks) {
     pdl_wait();
     pdl_next();
-    constexpr int LANES = 32 / VEC;
+    constexpr int LANES = 32 / (VEC * PIECES), STEP = 32 / PIECES;
     const int lane = threadIdx.x % LANES;
     const int64_t task = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     if (task >= tasks) return;                         // whole groups leave; the shuffles below stay inside a group
-    const uint32_t group = ((LANES == 32 ? 0u : 1u << LANES) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
+    const uint32_t group = ((1u << LANES) - 1) << (threadIdx.x & 31 & ~(LANES - 1));
     const int64_t quad = vec::quotient(task, by_blocks), r0 = quad * PACK_ROWS;
     const int b = (int)(task - quad * blocks), c = b * 32 + lane * VEC;
-    float v[PACK_ROWS][VEC];
+    vec::Piece<T, VEC> piece[PACK_ROWS][PIECES];
+    if (WHOLE)
 #pragma unroll
-    for (int u = 0; u < PACK_ROWS; u++) {
-        const bool live = r0 + u < n;
-        if (WHOLE) {
-            if (live && c < cols) vec::load<VEC>(x + (r0 + u) * ld + c, v[u]);
-            else
+        for (int u = 0; u < PACK_ROWS; u++)
 #pragma unroll
-                for (int i = 0; i < VEC; i++) v[u][i] = 0.f;
-        } else
-#pragma unroll
-            for (int i = 0; i < VEC; i++) v[u][i] = live && c + i < cols ? (float)x[(r0 + u) * ld + c + i] : 0.f;
-    }
+            for (int j = 0; j < PIECES; j++) piece[u][j].fetch(x + (r0 + u) * ld + c + j * STEP, r0 + u < n && c + j * STEP < cols);
     uint32_t s4 = 0;
 #pragma unroll
     for (int u = 0; u < PACK_ROWS; u++) {
+        float v[PIECES][VEC];
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            if (WHOLE) piece[u][j].values(v[j]);
+            else
+#pragma unroll
+                for (int i = 0; i < VEC; i++) v[j][i] = r0 + u < n && c + j * STEP + i < cols ? (float)x[(r0 + u) * ld + c + j * STEP + i] : 0.f;
+        }
         float most = 0.f;                              // NaN where there is one
 #pragma unroll
-        for (int i = 0; i < VEC; i++) most = max_magnitude(most, v[u][i]);
+        for (int j = 0; j < PIECES; j++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) most = max_magnitude(most, v[j][i]);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) most = max_magnitude(most, __shfl_xor_sync(group, most, o));
         const uint32_t top = __float_as_uint(most) & 0x7fffffffu;
@@ -82,26 +87,40 @@ __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ x, int6
         const bool bad = top >= 0x7f800000u;
         s4 |= (bad ? 255u : (uint32_t)(e + 127)) << (8 * u);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        uint32_t word[VEC / 4];
+        uint32_t word[PIECES][VEC / 4];
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4) {
-            uint32_t w = codes2(v[u][i] * down, v[u][i + 1] * down) | codes2(v[u][i + 2] * down, v[u][i + 3] * down) << 16;
-            // a byte of magnitude 0 (bit 7 of the sum stays clear) whose value is not: the smallest code
-            uint32_t some = 0;
+        for (int j = 0; j < PIECES; j++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) some |= v[u][i + k] != 0.f ? 1u << (8 * k) : 0;
-            w |= ~(((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) >> 7) & some;
-            // 256 * 2^120 and above are no float32: what rounds there takes 240 * 2^120
-            if (e == 120)
+            for (int i = 0; i < VEC; i += 4) {
+                uint32_t w = codes2(v[j][i] * down, v[j][i + 1] * down) | codes2(v[j][i + 2] * down, v[j][i + 3] * down) << 16;
+                // bytes of magnitude 0 (bit 7 of the sum stays clear) whose value is not: the smallest code
+                const uint32_t none = ~((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;
+                if (none) {
+                    uint32_t some = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if ((w >> (8 * k) & 0x7f) > 0x77) w = (w & ~(0x7fu << (8 * k))) | 0x77u << (8 * k);
-            word[i / 4] = bad ? 0x7f7f7f7fu : w;
-        }
+                    for (int k = 0; k < 4; k++) some |= v[j][i + k] != 0.f ? 1u << (8 * k) : 0;
+                    w |= none >> 7 & some;
+                }
+                word[j][i / 4] = w;
+            }
+        // 256 * 2^120 and above are no float32: what rounds there takes 240 * 2^120.  A block with infinity or NaN has 0x7f throughout.
+        if (e == 120 || bad)
+#pragma unroll
+            for (int j = 0; j < PIECES; j++)
+#pragma unroll
+                for (int i = 0; i < VEC / 4; i++) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if ((word[j][i] >> (8 * k) & 0x7f) > 0x77) word[j][i] = (word[j][i] & ~(0x7fu << (8 * k))) | 0x77u << (8 * k);
+                    if (bad) word[j][i] = 0x7f7f7f7fu;
+                }
         if (r0 + u < n) {
-            uint8_t *to = codes + (r0 + u) * (int64_t)blocks * 32 + c;
-            if (VEC == 8) __stcs(reinterpret_cast<uint2 *>(to), make_uint2(word[0], word[VEC / 4 - 1]));
-            else __stcs(reinterpret_cast<uint32_t *>(to), word[0]);
+#pragma unroll
+            for (int j = 0; j < PIECES; j++) {
+                uint8_t *to = codes + (r0 + u) * (int64_t)blocks * 32 + c + j * STEP;
+                if (VEC == 8) __stcs(reinterpret_cast<uint2 *>(to), make_uint2(word[j][0], word[j][VEC / 4 - 1]));
+                else __stcs(reinterpret_cast<uint32_t *>(to), word[j][0]);
+            }
         }
     }
     // rows behind the last lie inside the pitch, which is a multiple of 16
@@ -610,12 +629,12 @@ extern "C" int agpt_b200_act8_pack(const void *d_x, int64_t ld, int type, uint8_
     const auto grid = [&](int lanes) { return (unsigned)((s.tasks + 256 / lanes - 1) / (256 / lanes)); };
     if (type == AGPT_KV_BF16) {
         const bool whole = cols % 8 == 0 && ld % 8 == 0 && vec::aligned(d_x, 16);
-        if (whole) pdl_launch(pack_kernel<bf16, 8, true>, grid(4), 256, 0, st, (const bf16 *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
-        else pdl_launch(pack_kernel<bf16, 4, false>, grid(8), 256, 0, st, (const bf16 *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
+        if (whole) pdl_launch(pack_kernel<bf16, 8, 1, true>, grid(4), 256, 0, st, (const bf16 *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
+        else pdl_launch(pack_kernel<bf16, 4, 1, false>, grid(8), 256, 0, st, (const bf16 *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
     } else {
         const bool whole = cols % 4 == 0 && ld % 4 == 0 && vec::aligned(d_x, 16);
-        if (whole) pdl_launch(pack_kernel<float, 4, true>, grid(8), 256, 0, st, (const float *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
-        else pdl_launch(pack_kernel<float, 4, false>, grid(8), 256, 0, st, (const float *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
+        if (whole) pdl_launch(pack_kernel<float, 4, 2, true>, grid(4), 256, 0, st, (const float *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
+        else pdl_launch(pack_kernel<float, 4, 1, false>, grid(8), 256, 0, st, (const float *)d_x, ld, d_codes, d_scales, n, cols, s.blocks, s.pitch, by, s.tasks);
     }
     return launch_status("act8_pack");
 }
