@@ -12,13 +12,18 @@
 #include "../../include/agpt_b200.h"
 #include "internal.h"
 #include "pdl.cuh"
+#include "tc100.cuh"
 #include "vec.cuh"
 
 namespace {
 
 using bf16 = __nv_bfloat16;
+using tc::f2;
+using tc::f2_add; using tc::f2_fma; using tc::f2_get; using tc::f2_mul; using tc::f2_pack; using tc::f2_same;
 
-constexpr int BACK_BLOCKS = 4;         // blocks of the backward on an SM: 674 us at 1.4M x 8 x 32 in float32, with three 711 (the registers of a few spill)
+// Blocks of the backward on an SM by the bytes of an element of x: in float32 four (674 us at 1.4M x 8 x 32, three 711), in bfloat16, with eight columns a lane, three
+constexpr int back_blocks(int bytes) { return bytes == 4 ? 4 : 3; }
+
 
 struct Rows {                          // queries or keys: heads * head_dim columns, rows ld elements apart
     const void *x, *dy;
@@ -67,6 +72,13 @@ template <int VEC> __device__ __forceinline__ void load_cached(const float *p, f
         for (int i = 0; i < VEC; i++) v[i] = __ldg(p + i);
     }
 }
+// a piece as pairs of neighbouring columns: two columns an instruction, and the two that turn together
+template <typename T, int VEC> __device__ __forceinline__ void pairs(const vec::Piece<T, VEC> &p, f2 (&v)[VEC / 2]) {
+    float x[VEC];
+    p.values(x);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; i++) v[i] = f2_pack(x[2 * i], x[2 * i + 1]);
+}
 template <int VEC> __device__ __forceinline__ void load_gain(const float *gain, int c, float (&v)[VEC]) {
     if (gain) load_cached<VEC>(gain + c, v);
     else
@@ -100,21 +112,22 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
             piece[u][k].fetch(x + h * hd + c, live && h < m.heads && c < hd);
         }
     }
-    // entries 2 i of the tables, with the gain of both columns of the pair: y = (x0 r g0) cos - (x1 r g1) sin, (x0 r g0) sin + (x1 r g1) cos
-    float cs[NV][VEC / 2], sn[NV][VEC / 2], gain[NV][VEC];
+    // y = r (x0 g0 cos - x1 g1 sin, x0 g0 sin + x1 g1 cos): gain and table are multiplied once for all heads of the group
+    float2 from0[NV][VEC / 2], from1[NV][VEC / 2];
     const int at = live ? min(max(__ldg(P.pos + row), 0), P.n_pos - 1) : 0;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int c = (lane + k * lanes) * VEC;
         if (c >= hd) continue;
-        float t[VEC];
-        load_cached<VEC>(P.cosv + (int64_t)at * hd + c, t);
+        float cs[VEC], sn[VEC], gain[VEC];
+        load_cached<VEC>(P.cosv + (int64_t)at * hd + c, cs);
+        load_cached<VEC>(P.sinv + (int64_t)at * hd + c, sn);
+        load_gain<VEC>(m.gain, c, gain);
 #pragma unroll
-        for (int i = 0; i < VEC / 2; i++) cs[k][i] = t[2 * i];
-        load_cached<VEC>(P.sinv + (int64_t)at * hd + c, t);
-#pragma unroll
-        for (int i = 0; i < VEC / 2; i++) sn[k][i] = t[2 * i];
-        load_gain<VEC>(m.gain, c, gain[k]);
+        for (int i = 0; i < VEC; i += 2) {
+            from0[k][i / 2] = make_float2(gain[i] * cs[i], gain[i] * sn[i]);
+            from1[k][i / 2] = make_float2(-gain[i + 1] * sn[i], gain[i + 1] * cs[i]);
+        }
     }
     float r[HEADS], v[HEADS][NV][VEC];
 #pragma unroll
@@ -139,10 +152,10 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
             if (c >= hd) break;
             float y[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; i += 2) {
-                const float a = v[u][k][i] * r[u] * gain[k][i], b = v[u][k][i + 1] * r[u] * gain[k][i + 1];
-                y[i] = a * cs[k][i / 2] - b * sn[k][i / 2];
-                y[i + 1] = a * sn[k][i / 2] + b * cs[k][i / 2];
+            for (int i = 0; i < VEC / 2; i++) {
+                const float a = v[u][k][2 * i], b = v[u][k][2 * i + 1];
+                y[2 * i] = r[u] * (a * from0[k][i].x + b * from1[k][i].x);
+                y[2 * i + 1] = r[u] * (a * from0[k][i].y + b * from1[k][i].y);
             }
             store_either<VEC>(m.out, row * m.ld_out + h * hd + c, m.wide_out, y);
         }
@@ -152,7 +165,7 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const __grid_constant__ 
 // The blocks walk the tasks by a multiple of the groups of a row, so that a thread stays with its heads: side, gain and the columns' gain gradients are its own
 // for the whole kernel, and the row moves by a constant.  The block adds its groups in order into partial[block].
 template <typename T, typename D, int VEC, int NV, int HEADS, int LOG2>
-__global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_backward_kernel(const __grid_constant__ Heads P, const int64_t row_step) {
+__global__ void __launch_bounds__(256, NV == 1 ? back_blocks(sizeof(T)) : 1) norm_rope_backward_kernel(const __grid_constant__ Heads P, const int64_t row_step) {
     pdl_wait();
     pdl_next();
     extern __shared__ float s_gain[];                  // [groups of the block][2][hd]
@@ -164,13 +177,16 @@ __global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_back
     const bool is_q = g < P.q.groups;
     const Rows &m = is_q ? P.q : P.k;
     if (!is_q) g -= P.q.groups;
-    float sum[NV][VEC], gain[NV][VEC];
+    f2 sum[NV][VEC / 2], gain[NV][VEC / 2];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int c = (lane + k * lanes) * VEC;
+        float e[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) sum[k][i] = gain[k][i] = 0.f;
-        if (c < hd) load_gain<VEC>(m.gain, c, gain[k]);
+        for (int i = 0; i < VEC; i++) e[i] = 0.f;
+        if (c < hd) load_gain<VEC>(m.gain, c, e);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) { sum[k][i] = 0; gain[k][i] = f2_pack(e[2 * i], e[2 * i + 1]); }
     }
     const int64_t rounds = (P.n + row_step - 1) / row_step;
     int next = first < P.n ? __ldg(P.pos + first) : 0;     // the table waits for the position: asked for a round ahead
@@ -211,27 +227,23 @@ __global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_back
 #pragma unroll
         for (int u = 0; u < HEADS; u++) {
             const int h = g + u * m.groups;
-            float sq = 0.f, dot = 0.f, x[NV][VEC], d[NV][VEC];
-            // d becomes w = R^T dy
+            f2 sq = 0, dot = 0, x[NV][VEC / 2], w[NV][VEC / 2];
 #pragma unroll
             for (int k = 0; k < NV; k++) {
-                x_piece[u][k].values(x[k]);
-                d_piece[u][k].values(d[k]);
+                float d[VEC];
+                pairs(x_piece[u][k], x[k]);
+                d_piece[u][k].values(d);
 #pragma unroll
-                for (int i = 0; i < VEC; i += 2) {
-                    const float a = d[k][i], b = d[k][i + 1], co = cs[k][i / 2], si = sn[k][i / 2];
-                    d[k][i] = a * co + b * si;
-                    d[k][i + 1] = b * co - a * si;
-                }
-#pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    sq += x[k][i] * x[k][i];
-                    dot += d[k][i] * gain[k][i] * x[k][i];
+                for (int i = 0; i < VEC / 2; i++) {
+                    const float a = d[2 * i], b = d[2 * i + 1];
+                    w[k][i] = f2_pack(a * cs[k][i] + b * sn[k][i], b * cs[k][i] - a * sn[k][i]);
+                    sq = f2_fma(x[k][i], x[k][i], sq);
+                    dot = f2_fma(f2_mul(w[k][i], gain[k][i]), x[k][i], dot);
                 }
             }
-            sq = group_sum<LOG2>(sq, lanes);
-            dot = group_sum<LOG2>(dot, lanes);
-            const float r = rsqrtf(sq * P.inv_hd + P.eps), f = r * r * (dot * P.inv_hd);
+            const float2 sq2 = f2_get(sq), dot2 = f2_get(dot);
+            const float square = group_sum<LOG2>(sq2.x + sq2.y, lanes), product = group_sum<LOG2>(dot2.x + dot2.y, lanes);
+            const float r = rsqrtf(square * P.inv_hd + P.eps), f = r * r * (product * P.inv_hd);
             if (!live || h >= m.heads) continue;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
@@ -239,9 +251,10 @@ __global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_back
                 if (c >= hd) break;
                 float y[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    y[i] = r * (d[k][i] * gain[k][i] - x[k][i] * f);
-                    sum[k][i] += d[k][i] * (x[k][i] * r);
+                for (int i = 0; i < VEC / 2; i++) {
+                    const float2 t = f2_get(f2_mul(f2_fma(x[k][i], f2_same(-f), f2_mul(w[k][i], gain[k][i])), f2_same(r)));
+                    y[2 * i] = t.x; y[2 * i + 1] = t.y;
+                    sum[k][i] = f2_fma(w[k][i], f2_mul(x[k][i], f2_same(r)), sum[k][i]);
                 }
                 store_either<VEC>(m.out, row * m.ld_out + h * hd + c, m.wide_out, y);
             }
@@ -254,7 +267,8 @@ __global__ void __launch_bounds__(256, NV == 1 ? BACK_BLOCKS : 1) norm_rope_back
         if (c < hd)
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                s_gain[(own * 2 + !is_q) * hd + c + i] = sum[k][i];
+                const float2 t = f2_get(sum[k][i / 2]);
+                s_gain[(own * 2 + !is_q) * hd + c + i] = i & 1 ? t.y : t.x;
                 s_gain[(own * 2 + is_q) * hd + c + i] = 0.f;
             }
     }
@@ -311,13 +325,13 @@ void split(Heads &P, int vec, int heads_each, int low) {
     P.tasks = P.n * P.groups;
 }
 // Blocks of the backward: as many as run at once, in a number that makes their tasks a multiple of the groups of a row.
-int64_t most_blocks() { return (int64_t)vec::sm_count() * BACK_BLOCKS; }
-int backward_blocks(const Heads &P) {
+int64_t most_blocks(int bytes) { return (int64_t)vec::sm_count() * back_blocks(bytes); }
+int backward_blocks(const Heads &P, int bytes) {
     const int per_block = 256 >> P.lanes_log2;
     int step = P.groups;                               // groups / gcd(groups, per_block), per_block a power of two
     for (int b = per_block; b > 1 && step % 2 == 0; b /= 2) step /= 2;
     // two rounds a block at least: a block costs a row of partial sums and its start
-    const int64_t want = (P.tasks + 2 * per_block - 1) / (2 * per_block), rounded = (want + step - 1) / step * step, most = most_blocks() / step * step;
+    const int64_t want = (P.tasks + 2 * per_block - 1) / (2 * per_block), rounded = (want + step - 1) / step * step, most = most_blocks(bytes) / step * step;
     return (int)(rounded < most ? rounded : most < step ? step : most);
 }
 
@@ -341,7 +355,7 @@ int forward(Heads &P, cudaStream_t st) {
 template <typename T, typename D, int VEC, int NV, int LOW>
 int backward(Heads &P, float *dq_gain, float *dk_gain, cudaStream_t st) {
     split(P, VEC, BACK_HEADS, LOW);
-    const int blocks = backward_blocks(P), per_block = 256 >> P.lanes_log2;
+    const int blocks = backward_blocks(P, sizeof(T)), per_block = 256 >> P.lanes_log2;
     const size_t smem = P.partial ? (size_t)per_block * 2 * P.hd * 4 : 0;
     const int64_t row_step = (int64_t)blocks * per_block / P.groups;
     const auto go = [&](void (*kernel)(const Heads, const int64_t)) { pdl_launch(kernel, (unsigned)blocks, 256, smem, st, P, row_step); };
@@ -390,7 +404,7 @@ extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void 
 
 extern "C" int64_t agpt_b200_qk_norm_rope_backward_workspace_bytes(int head_dim) {
     if (head_dim < 2 || head_dim > 256) return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward_workspace_bytes: bad argument");
-    return (most_blocks() + MAX_HEADS) * 2 * head_dim * 4;
+    return (most_blocks(4) + MAX_HEADS) * 2 * head_dim * 4;
 }
 
 extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, const void *d_dk, int64_t dk_ld, int grad_type, const void *d_q, int64_t q_ld,
