@@ -188,6 +188,26 @@ __global__ void __launch_bounds__(256, NV == 1 ? back_blocks(sizeof(T)) : 1) nor
 #pragma unroll
         for (int i = 0; i < VEC / 2; i++) { sum[k][i] = 0; gain[k][i] = f2_pack(e[2 * i], e[2 * i + 1]); }
     }
+    // A float32 sum over thousands of rows one after the other loses bits: every FLUSH rounds it goes to the thread's own place in shared memory.
+    constexpr int FLUSH = 32;
+    const auto flush = [&](bool first_time) {
+        if (!P.partial) return;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int c = (lane + k * lanes) * VEC;
+            if (c < hd)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    const float2 t = f2_get(sum[k][i / 2]);
+                    float *mine = s_gain + (own * 2 + !is_q) * hd + c + i;
+                    *mine = first_time ? 0.f : *mine + (i & 1 ? t.y : t.x);
+                    if (first_time) s_gain[(own * 2 + is_q) * hd + c + i] = 0.f;
+                }
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) sum[k][i] = 0;
+        }
+    };
+    flush(true);
     const int64_t rounds = (P.n + row_step - 1) / row_step;
     int next = first < P.n ? __ldg(P.pos + first) : 0;     // the table waits for the position: asked for a round ahead
     for (int64_t t = 0; t < rounds; t++) {
@@ -259,19 +279,10 @@ __global__ void __launch_bounds__(256, NV == 1 ? back_blocks(sizeof(T)) : 1) nor
                 store_either<VEC>(m.out, row * m.ld_out + h * hd + c, m.wide_out, y);
             }
         }
+        if (t % FLUSH == FLUSH - 1) flush(false);
     }
     if (!P.partial) return;
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const int c = (lane + k * lanes) * VEC;
-        if (c < hd)
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float2 t = f2_get(sum[k][i / 2]);
-                s_gain[(own * 2 + !is_q) * hd + c + i] = i & 1 ? t.y : t.x;
-                s_gain[(own * 2 + is_q) * hd + c + i] = 0.f;
-            }
-    }
+    flush(false);
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * hd; c += 256) {
         float s = 0.f;
