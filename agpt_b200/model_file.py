@@ -74,6 +74,39 @@ def save(path: str, m: Model) -> None:
             f.write(a.tobytes())
 
 
+# Gains of the query and key norms, which the model file has no place for: a file beside it, u32 magic, i32 count, then
+# matrices [1, head_dim] as in the model file, per layer those of the queries and of the keys.
+GAINS_MAGIC, GAINS_SUFFIX = 0x4E474B51, ".qk_gains"
+
+
+def load_gains(path: str, n_layers: int, head_dim: int):
+    """{name: float32 [1, head_dim]} of a gains file."""
+    with open(path, "rb") as f:
+        raw = f.read()
+    if len(raw) != 8 + 2 * n_layers * (8 + 4 * head_dim) or struct.unpack_from("<Ii", raw, 0) != (GAINS_MAGIC, 2 * n_layers):
+        raise ValueError(f"{path}: not the query and key gains of {n_layers} layers with heads of {head_dim}")
+    out, off = {}, 8
+    for name in gain_names(n_layers):
+        if struct.unpack_from("<2i", raw, off) != (1, head_dim):
+            raise ValueError(f"{path}: {name} is not 1x{head_dim}")
+        out[name] = np.frombuffer(raw, dtype="<f4", count=head_dim, offset=off + 8).reshape(1, head_dim).copy()
+        off += 8 + 4 * head_dim
+    return out
+
+
+def save_gains(path: str, gains) -> None:
+    with open(path, "wb") as f:
+        f.write(struct.pack("<Ii", GAINS_MAGIC, len(gains)))
+        for a in gains.values():
+            a = np.ascontiguousarray(a, dtype="<f4")
+            f.write(struct.pack("<2i", 1, a.size))
+            f.write(a.tobytes())
+
+
+def gain_names(n_layers: int):
+    return [f"layer{l}.{n}.gain" for l in range(n_layers) for n in ("qn", "kn")]
+
+
 def random_init(d_model, n_heads, n_layers, vocab, seq_len, d_ff=None, seed=0, std=0.02) -> Model:
     """Seeded N(0, std) weights, gamma 1, beta and biases 0, in file order."""
     d_ff = 4 * d_model if d_ff is None else d_ff

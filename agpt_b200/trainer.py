@@ -169,6 +169,26 @@ def _embedding_function():
     return TokenEmbedding
 
 
+def _scaled_embedding_function():
+    import torch
+
+    class ScaledEmbedding(torch.autograd.Function):
+        """Rows of the token table times a scale, for vocabularies of any size: the gradient is summed over the rows in the order of their tokens."""
+
+        @staticmethod
+        def forward(ctx, emb, tokens32, scale):
+            ctx.save_for_backward(tokens32)
+            ctx.vocab, ctx.scale = emb.shape[0], scale
+            return A.embedding_lookup(emb, tokens32, scale)
+
+        @staticmethod
+        def backward(ctx, grad):
+            (tokens32,) = ctx.saved_tensors
+            return A.embedding_grad_sorted(grad.contiguous(), tokens32, ctx.vocab, ctx.scale), None, None
+
+    return ScaledEmbedding
+
+
 def _layer_norm_function():
     import torch
 
@@ -255,6 +275,66 @@ def _qkv_function():
     return QKVProjection
 
 
+def _kept8(ctx):
+    """The 8-bit activations a function has saved (codes and scales, pair by pair) and the tensors behind them."""
+    t = ctx.saved_tensors
+    return [A.Act8(t[2 * i], t[2 * i + 1], c) for i, c in enumerate(ctx.kept_cols)], t[2 * len(ctx.kept_cols):]
+
+
+def _keep8(ctx, kept, *tensors):
+    ctx.kept_cols = [a.cols for a in kept]
+    ctx.save_for_backward(*[t for a in kept for t in (a.codes, a.scales)], *tensors)
+
+
+def _qkv8_function():
+    import torch
+
+    class QKVProjection8(torch.autograd.Function):
+        """QKVProjection whose input is kept in 8 bits: the weight gradients are formed from the kept values, everything else is the same."""
+
+        @staticmethod
+        def forward(ctx, x, wq, bq, wk, bk, wv, bv):
+            x = x.contiguous()
+            _keep8(ctx, [A.act8_pack(x)], wq, wk, wv)
+            return A.gemm_f32(x, wq, bias=bq), A.gemm_f32(x, wk, bias=bk), A.gemm_f32(x, wv, bias=bv)
+
+        @staticmethod
+        def backward(ctx, dq, dk, dv):
+            (x8,), weights = _kept8(ctx)
+            dx, out = None, []
+            for g, w in zip((dq, dk, dv), weights):
+                g = g.contiguous()
+                dx = A.gemm_f32(g, w, trans_b=True, residual=dx, out=dx)
+                out += A.act8_weight_grad(x8, g)
+            return (dx, *out)
+
+    return QKVProjection8
+
+
+def _ffn8_function():
+    import torch
+
+    class FeedForward8(torch.autograd.Function):
+        """relu(x W1 + b1) W2 + b2 + residual with both projections' inputs kept in 8 bits; the mask of the ReLU is read from the second one's codes."""
+
+        @staticmethod
+        def forward(ctx, x, w1, b1, w2, b2, residual):
+            x = x.contiguous()
+            h = A.gemm_f32(x, w1, bias=b1, relu=True)
+            _keep8(ctx, [A.act8_pack(x), A.act8_pack(h)], w1, w2)
+            return A.gemm_f32(h, w2, bias=b2, residual=residual.contiguous())
+
+        @staticmethod
+        def backward(ctx, grad):
+            (x8, h8), (w1, w2) = _kept8(ctx)
+            grad = grad.contiguous()
+            dh = A.gemm_f32(grad, w2, trans_b=True)
+            dh = A.act8_relu_backward(dh, h8, out=dh)
+            return (A.gemm_f32(dh, w1, trans_b=True), *A.act8_weight_grad(x8, dh), *A.act8_weight_grad(h8, grad), grad)
+
+    return FeedForward8
+
+
 def _linear_function():
     import torch
 
@@ -313,31 +393,71 @@ def _attention_function():
     return TrieAttention
 
 
-class TrieWalkModel:
-    """Parameters of an MGPT model as torch tensors on one device, and the per-group forward/backward."""
+def _norm_attention_function():
+    import torch
 
-    def __init__(self, model: MF.Model, device):
+    class NormTrieAttention(torch.autograd.Function):
+        """TrieAttention behind an RMS norm of queries and keys per head, norm and rotation in one pass; keys go straight into a bfloat16 store."""
+
+        @staticmethod
+        def forward(ctx, q, k, v, q_gain, k_gain, group, cos, sin, n_heads, bf16_store, grad_mode="full"):
+            q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+            qr, ks = A.qk_norm_rope(q, k, q_gain, k_gain, group.pos, cos, sin, k_dtype=torch.bfloat16 if bf16_store else None)
+            vs = A.kv_store_write_bf16(v) if bf16_store else v
+            out, lse = A.attn_forward(group.plan, qr, ks, vs, n_heads)
+            ctx.save_for_backward(q, k, q_gain, k_gain, qr, ks, vs, out, lse)
+            ctx.group, ctx.cos, ctx.sin, ctx.n_heads, ctx.grad_mode = group, cos, sin, n_heads, grad_mode
+            return out
+
+        @staticmethod
+        def backward(ctx, dout):
+            q, k, q_gain, k_gain, qr, ks, vs, out, lse = ctx.saved_tensors
+            dq, dk, dv = A.attn_backward(ctx.group.plan, qr, ks, vs, out, lse, dout.contiguous(), ctx.n_heads, grad_mode=ctx.grad_mode,
+                                         edge_first=ctx.group.edge_first)
+            dqg, dkg = torch.zeros_like(q_gain), torch.zeros_like(k_gain)
+            A.qk_norm_rope_backward(dq, dk, q, k, q_gain, k_gain, ctx.group.pos, ctx.cos, ctx.sin, dqg, dkg, q_out=dq, k_out=dk)
+            return dq, dk, dv, dqg, dkg, None, None, None, None, None, None
+
+    return NormTrieAttention
+
+
+# symbols the embedding gradient in shared memory (and the native step) takes; larger vocabularies go by sorted tokens
+TABLE_VOCAB = 400
+
+
+class TrieWalkModel:
+    """Parameters of an MGPT model as torch tensors on one device, and the per-group forward/backward.
+
+    Beyond the reference's model, each off by default and stepped on the tape: qk_norm (queries and keys normalised per head, with gains that follow the
+    file's matrices in the flat buffers), embed_scale (a factor on the embedding) and, as an attribute, activations_8bit (the inputs of the q/k/v and
+    feed-forward projections are kept for the backward in 8 bits)."""
+
+    def __init__(self, model: MF.Model, device, qk_norm: bool = False, embed_scale: float = 1.0):
         import torch
         self.cfg = model
         self.device = device
+        self.qk_norm, self.embed_scale, self.activations_8bit = bool(qk_norm), float(embed_scale), False
+        hd = model.d_model // model.n_heads
+        mats = list(model.mats)
+        if qk_norm:
+            mats += [(name, np.ones((1, hd), np.float32)) for name in MF.gain_names(model.n_layers)]
         # one flat weight buffer and one flat gradient buffer (the reference's d_weights / d_grads), each matrix on a
         # 16-byte boundary; the gradient buffer ends with the epoch's loss sum and query count (three floats) and the device status so that
         # one all-reduce carries everything
         offs, off = [], 0
-        for _, a in model.mats:
+        for _, a in mats:
             offs.append(off)
             off += (a.size + 3) & ~3
         self.n_flat = off
         self.flat = torch.zeros(off, dtype=torch.float32, device=device)
         self.flat_grad = torch.zeros(off + 4, dtype=torch.float32, device=device)
         self.params = {}
-        for (name, a), o in zip(model.mats, offs):
+        for (name, a), o in zip(mats, offs):
             p = self.flat[o:o + a.size].view(a.shape)
             p.copy_(torch.from_numpy(np.ascontiguousarray(a)))
             self.params[name] = p.requires_grad_(True)
-        self._offs, self._shapes = offs, [torch.Size(a.shape) for _, a in model.mats] * 2
+        self._offs, self._shapes = offs, [torch.Size(a.shape) for _, a in mats] * 2
         self.bind_grads()
-        hd = model.d_model // model.n_heads
         cos, sin = A.rope_table(model.seq_len, hd)
         self.cos, self.sin = torch.from_numpy(cos).to(device), torch.from_numpy(sin).to(device)
         self.attn = _attention_function()
@@ -346,6 +466,8 @@ class TrieWalkModel:
         self.linear = _linear_function()
         self.norm_skip = _norm_skip_function()
         self.qkv = _qkv_function()
+        self.scaled_embed, self.norm_attn = _scaled_embedding_function(), _norm_attention_function()
+        self.qkv8, self.ffn8 = _qkv8_function(), _ffn8_function()
         self.dense_impl = "tensor"       # "tensor": the library's kernels; "torch": torch.addmm (cuBLAS float32)
         self.ffn_recompute = False       # True: recompute the d_ff-wide activations in the backward instead of keeping them
         # which attention pairs feed dK/dV: "full" (persistent accumulators, src/agpt/incremental_backward.cr), "local_depth"
@@ -368,6 +490,16 @@ class TrieWalkModel:
         out.mats = [(name, self.params[name].detach().cpu().numpy().copy()) for name, _ in m.mats]
         return out
 
+    def qk_gains(self):
+        """The gains of the query and key norms by name, float32 [1, head_dim] (none without them): what MF.save_gains writes beside the model file."""
+        return {name: self.params[name].detach().cpu().numpy().copy() for name in MF.gain_names(self.cfg.n_layers)} if self.qk_norm else {}
+
+    def set_qk_gains(self, gains):
+        import torch
+        with torch.no_grad():
+            for name, a in gains.items():
+                self.params[name].copy_(torch.from_numpy(np.ascontiguousarray(a)))
+
     def logits(self, group: LaunchGroup, bf16_store=False):
         import torch
         from torch.utils.checkpoint import checkpoint
@@ -386,25 +518,34 @@ class TrieWalkModel:
             return lin(lin(ln(x, g2, b2), w1, b1, relu=True), w2, bo, residual=x)
 
         fused = self.dense_impl == "tensor" and m.d_model % 4 == 0 and m.d_ff % 4 == 0
-        x = self.embed.apply(P["token_emb"], group.tokens32, group.even)
+        eight = self.activations_8bit
+        if eight and (not fused or self.ffn_recompute):
+            raise A.AgptError("8-bit activations go with the library's projections (widths that are multiples of 4) and not with recomputed ones")
+        if m.vocab > TABLE_VOCAB or self.embed_scale != 1.0:
+            x = self.scaled_embed.apply(P["token_emb"], group.tokens32, self.embed_scale)
+        else:
+            x = self.embed.apply(P["token_emb"], group.tokens32, group.even)
         for l in range(m.n_layers):
             g = lambda n: P[f"layer{l}.{n}"]  # noqa: E731
             if fused:
                 x1, skip = self.norm_skip.apply(x, g("ln1.gamma")[0], g("ln1.beta")[0])
-                q, k, v = self.qkv.apply(x1, g("wq.w"), g("wq.b")[0], g("wk.w"), g("wk.b")[0], g("wv.w"), g("wv.b")[0])
+                q, k, v = (self.qkv8 if eight else self.qkv).apply(x1, g("wq.w"), g("wq.b")[0], g("wk.w"), g("wk.b")[0], g("wv.w"), g("wv.b")[0])
             else:
                 x1, skip = ln(x, g("ln1.gamma")[0], g("ln1.beta")[0]), x
                 q = lin(x1, g("wq.w"), g("wq.b")[0])
                 k = lin(x1, g("wk.w"), g("wk.b")[0])
                 v = lin(x1, g("wv.w"), g("wv.b")[0])
-            a = self.attn.apply(q, k, v, group, self.cos, self.sin, m.n_heads, bf16_store, self.grad_mode)
+            if self.qk_norm:
+                a = self.norm_attn.apply(q, k, v, g("qn.gain")[0], g("kn.gain")[0], group, self.cos, self.sin, m.n_heads, bf16_store, self.grad_mode)
+            else:
+                a = self.attn.apply(q, k, v, group, self.cos, self.sin, m.n_heads, bf16_store, self.grad_mode)
             x = lin(a, g("wo.w"), g("wo.b")[0], residual=skip)
             args = (x, g("ln2.gamma")[0], g("ln2.beta")[0], g("l1.w"), g("l1.b")[0], g("l2.w"), g("l2.b")[0])
             if self.ffn_recompute:
                 x = checkpoint(ffn, *args, use_reentrant=False)
             elif fused:
                 x2, skip = self.norm_skip.apply(x, args[1], args[2])
-                x = lin(lin(x2, args[3], args[4], relu=True), args[5], args[6], residual=skip)
+                x = self.ffn8.apply(x2, *args[3:], skip) if eight else lin(lin(x2, args[3], args[4], relu=True), args[5], args[6], residual=skip)
             else:
                 x = ffn(*args)
         xf = ln(x, P["final.gamma"][0], P["final.beta"][0])
@@ -422,6 +563,8 @@ class TrieWalkModel:
 
     def native_step_available(self) -> bool:
         m = self.cfg
+        if self.qk_norm or self.embed_scale != 1.0 or self.activations_8bit:
+            return False                                         # the native step has none of them
         return self.dense_impl == "tensor" and bool(A.lib().agpt_b200_train_step_takes(m.d_model, m.n_heads, m.d_ff, m.vocab))
 
     def _step_addresses(self):
@@ -721,6 +864,10 @@ def main(argv=None):
     ap.add_argument("--grad-mode", default="full", choices=["full", "local_depth", "own_edge"],
                     help="attention pairs that feed dK/dV: every descendant (default), the node's own query, or the queries on the key's radix edge")
     ap.add_argument("--group-rows", type=int, default=1_000_000)
+    ap.add_argument("--qk-norm", action="store_true", help="RMS norm of queries and keys per head, with gains kept in a file beside the model's (MODEL.qk_gains)")
+    ap.add_argument("--embed-scale", type=float, default=1.0, help="factor on the embedding rows")
+    ap.add_argument("--activations-8bit", action="store_true",
+                    help="keep the inputs of the q/k/v and feed-forward projections in 8 bits for the backward (less memory)")
     ap.add_argument("--ffn-recompute", action="store_true", help="recompute the FFN activations in the backward (less memory)")
     ap.add_argument("--lightning-sampler", default=None, choices=["l1", "l2", "l3", "l4"],
                     help="stochastic training units instead of the deterministic sweep (one rank)")
@@ -732,6 +879,8 @@ def main(argv=None):
     ap.add_argument("--partition-depth", type=int, default=0, choices=[0, 1, 2],
                     help="1 = root-child units, 2 = bigram units; 0 = 1 on one rank, 2 on several")
     args = ap.parse_args(argv)
+    if args.activations_8bit and args.ffn_recompute:
+        ap.error("--activations-8bit keeps what --ffn-recompute would form again: choose one")
 
     world, rank, local = (int(os.environ.get(k, d)) for k, d in (("WORLD_SIZE", "1"), ("RANK", "0"), ("LOCAL_RANK", "0")))
     if not torch.cuda.is_available():
@@ -755,14 +904,23 @@ def main(argv=None):
                                      level=args.partition_depth or None)
     rng_state = args.lightning_seed
     counts = [torch.tensor(c, dtype=torch.int32, device=dev) for c in (trie.cnt_off, trie.cnt_tok, trie.cnt_val)]
-    model = TrieWalkModel(mf, dev)
-    model.ffn_recompute = args.ffn_recompute
+    model = TrieWalkModel(mf, dev, args.qk_norm, args.embed_scale)
+    if os.path.exists(args.model + MF.GAINS_SUFFIX):
+        if not args.qk_norm:
+            raise SystemExit(f"{args.model + MF.GAINS_SUFFIX} lies beside the model: it was trained with --qk-norm")
+        model.set_qk_gains(MF.load_gains(args.model + MF.GAINS_SUFFIX, mf.n_layers, mf.d_model // mf.n_heads))
+    model.ffn_recompute, model.activations_8bit = args.ffn_recompute, args.activations_8bit
     model.grad_mode = args.grad_mode
     opt = make_optimizer(args.optimizer, model, args.lr, args.rmsprop_beta, weight_decay=args.weight_decay,
                          clip_norm=args.grad_clip_norm)
     n_sub = int((trie.parent[1:] == 0).sum())
     # optimizer steps per epoch, as the reference counts them for its schedule (src/cuda/agpt_train.cu:5100-5117)
     per_epoch = args.lightning_steps if lightning else (len(groups) if (args.no_accumulate and world == 1) else 1)
+    def save_model(path):
+        MF.save(path, model.to_model_file())
+        if model.qk_norm:
+            MF.save_gains(path + MF.GAINS_SUFFIX, model.qk_gains())
+
     if args.lr_schedule != "constant":
         opt.schedule = (args.lr_schedule, max(per_epoch * args.epochs, 1), args.warmup_epochs * per_epoch)
     save = args.save or args.model
@@ -784,9 +942,9 @@ def main(argv=None):
             print(f"Epoch {ep}: loss={ls / max(nq, 1):.6f}  ({time.time() - t0:.2f} sec, {units} subtrees, {chunks} chunks, {nq} nodes)",
                   flush=True)
             if args.save_every and ep % args.save_every == 0:
-                MF.save(f"{save}.ep{ep}", model.to_model_file())
+                save_model(f"{save}.ep{ep}")
     if rank == 0:
-        MF.save(save, model.to_model_file())
+        save_model(save)
     if world > 1:
         dist.destroy_process_group()
 
