@@ -760,7 +760,8 @@ def embedding_grad(grad, ids32, vocab, out=None, accumulate=False, serial=False)
 class _Runtime:
     def __init__(self):
         import torch
-        self.torch = torch
+        self.torch, self.lib, self.empty_like, self.empty = torch, lib(), torch.empty_like, torch.empty
+        self.u8, self.f32, self.i32 = torch.uint8, torch.float32, torch.int32
         self.kinds = {torch.float32: KV_F32, torch.bfloat16: KV_BF16}
         self.ids = {torch.int32: 0, torch.int64: 1}
         self.current_device, self.stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -803,6 +804,11 @@ def _rows_like(rt, t, name, kind, n, cols, dev, whole=False):
     return ld
 
 
+def _new_rows(rt, t, n, cols, ld):
+    """A contiguous tensor of the shape, type and device of t, whose rows are ld elements apart."""
+    return rt.empty_like(t) if ld == cols else t.new_empty((n, cols))
+
+
 def _flat(t, name, dtype, numel, dev):
     """Address of a contiguous tensor of a known type, size and device; None stays None."""
     if t is None:
@@ -832,7 +838,7 @@ def _scratch_for(rt, t, dev, what, fn, *args):
         if len(rt.sizes) > 4096:
             rt.sizes.clear()
         rt.sizes[what, dev, args] = need
-    return (t.new_empty(need, dtype=rt.torch.uint8) if need else None), need
+    return (t.new_empty(need, dtype=rt.u8) if need else None), need
 
 
 def _ids(rt, ids, n, dev):
@@ -853,7 +859,7 @@ def embedding_lookup(emb, ids, scale: float = 1.0, out=None):
         out = emb.new_empty((n, d))
     else:
         _rows_like(rt, out, "out", kind, n, d, dev, whole=True)
-    _on(rt, dev, "embedding_lookup", lib().agpt_b200_embedding_lookup, emb.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), n, d, vocab, scale)
+    _on(rt, dev, "embedding_lookup", rt.lib.agpt_b200_embedding_lookup, emb.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), n, d, vocab, scale)
     return out
 
 
@@ -865,11 +871,11 @@ def embedding_grad_sorted(grad, ids, vocab: int, scale: float = 1.0, out=None, a
     kind, n, d, ld, dev = _rows(rt, grad, "grad")
     wide, out_kind = _ids(rt, ids, n, dev), KV_F32
     if out is None:
-        out = (grad.new_zeros if accumulate else grad.new_empty)((vocab, d), dtype=rt.torch.float32)
+        out = (grad.new_zeros if accumulate else grad.new_empty)((vocab, d), dtype=rt.f32)
     else:
         out_kind = rt.kinds.get(out.dtype)
         _rows_like(rt, out, "out", out_kind, vocab, d, dev, whole=True)
-    L = lib()
+    L = rt.lib
     ws, need = _scratch_for(rt, grad, dev, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted_workspace_bytes, n, d, vocab)
     _on(rt, dev, "embedding_grad_sorted", L.agpt_b200_embedding_grad_sorted, grad.data_ptr(), ld, kind, ids.data_ptr(), wide, out.data_ptr(), out_kind, n, d, vocab, scale,
         int(accumulate), None if ws is None else ws.data_ptr(), need)
@@ -878,11 +884,11 @@ def embedding_grad_sorted(grad, ids, vocab: int, scale: float = 1.0, out=None, a
 
 def _rope_tables(rt, pos, cos, sin, q_gain, k_gain, n, dev):
     """(head_dim, addresses of gains, positions and tables, positions in the tables)"""
-    f32, shape = rt.torch.float32, cos.shape
+    f32, shape = rt.f32, cos.shape
     if len(shape) != 2 or sin.shape != shape or not shape[0]:
         raise AgptError("cos and sin must be [positions, head_dim] tables")
     n_pos, hd = shape
-    return hd, (_flat(q_gain, "q_gain", f32, hd, dev), _flat(k_gain, "k_gain", f32, hd, dev), _flat(pos, "pos", rt.torch.int32, n, dev),
+    return hd, (_flat(q_gain, "q_gain", f32, hd, dev), _flat(k_gain, "k_gain", f32, hd, dev), _flat(pos, "pos", rt.i32, n, dev),
                 _flat(cos, "cos", f32, n_pos * hd, dev), _flat(sin, "sin", f32, n_pos * hd, dev), n_pos)
 
 
@@ -906,21 +912,24 @@ def qk_norm_rope(q, k, q_gain, k_gain, pos, cos, sin, eps: float = 1e-6, k_dtype
     q_kind = k_kind = kind
     qo_ld, ko_ld = qc, kc
     if q_out is None:
-        q_out = q.new_empty((n, qc))
+        q_out = _new_rows(rt, q, n, qc, q_ld)
     else:
         q_kind = rt.kinds.get(q_out.dtype)
         qo_ld = _rows_like(rt, q_out, "q_out", q_kind, n, qc, dev)
     if k_out is None:
-        k_out = k.new_empty((n, kc), dtype=k_dtype)
-        k_kind = rt.kinds.get(k_out.dtype)
-        if k_kind is None:
-            raise AgptError(f"k_dtype {k_dtype}: float32 or bfloat16")
+        if k_dtype is None or k_dtype is k.dtype:
+            k_out = _new_rows(rt, k, n, kc, k_ld)
+        else:
+            k_kind = rt.kinds.get(k_dtype)
+            if k_kind is None:
+                raise AgptError(f"k_dtype {k_dtype}: float32 or bfloat16")
+            k_out = k.new_empty((n, kc), dtype=k_dtype)
     else:
         if k_dtype is not None and k_out.dtype != k_dtype:
             raise AgptError(f"k_out has dtype {k_out.dtype}, k_dtype says {k_dtype}")
         k_kind = rt.kinds.get(k_out.dtype)
         ko_ld = _rows_like(rt, k_out, "k_out", k_kind, n, kc, dev)
-    _on(rt, dev, "qk_norm_rope", lib().agpt_b200_qk_norm_rope, q.data_ptr(), q_ld, k.data_ptr(), k_ld, kind, *tables, n, hq, hk, hd, eps, q_out.data_ptr(), qo_ld, q_kind,
+    _on(rt, dev, "qk_norm_rope", rt.lib.agpt_b200_qk_norm_rope, q.data_ptr(), q_ld, k.data_ptr(), k_ld, kind, *tables, n, hq, hk, hd, eps, q_out.data_ptr(), qo_ld, q_kind,
         k_out.data_ptr(), ko_ld, k_kind)
     return q_out, k_out
 
@@ -938,16 +947,16 @@ def qk_norm_rope_backward(dq, dk, q, k, q_gain, k_gain, pos, cos, sin, dq_gain=N
     hq, hk = _heads(qc, hd, "q"), _heads(kc, hd, "k")
     qo_ld, ko_ld = qc, kc
     if q_out is None:
-        q_out = q.new_empty((n, qc))
+        q_out = _new_rows(rt, q, n, qc, q_ld)
     else:
         qo_ld = _rows_like(rt, q_out, "q_out", kind, n, qc, dev)
     if k_out is None:
-        k_out = k.new_empty((n, kc))
+        k_out = _new_rows(rt, k, n, kc, k_ld)
     else:
         ko_ld = _rows_like(rt, k_out, "k_out", kind, n, kc, dev)
-    f32 = rt.torch.float32
+    f32 = rt.f32
     gains = _flat(dq_gain, "dq_gain", f32, hd, dev), _flat(dk_gain, "dk_gain", f32, hd, dev)
-    L, ws, need = lib(), None, 0
+    L, ws, need = rt.lib, None, 0
     if gains != (None, None):
         ws, need = _scratch_for(rt, q, dev, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward_workspace_bytes, hd)
     _on(rt, dev, "qk_norm_rope_backward", L.agpt_b200_qk_norm_rope_backward, dq.data_ptr(), dq_ld, dk.data_ptr(), dk_ld, grad_kind, q.data_ptr(), q_ld, k.data_ptr(), k_ld,
@@ -962,7 +971,7 @@ class Act8:
     __slots__ = ("codes", "scales", "cols")
 
     def __init__(self, codes, scales, cols: int):
-        u8, blocks = _rt().torch.uint8, (cols + 31) // 32
+        u8, blocks = _rt().u8, (cols + 31) // 32
         n, c = codes.shape if codes.dim() == 2 else (0, 0)
         if cols < 1 or c != blocks * 32 or codes.dtype is not u8 or scales.dtype is not u8 or scales.shape != (blocks, (n + 15) // 16 * 16) or not codes.is_contiguous() or \
                 not scales.is_contiguous():
@@ -988,18 +997,18 @@ def act8_pack(x) -> Act8:
     kind, n, cols, ld, dev = _rows(rt, x, "x")
     if not cols:
         raise AgptError("x has no columns")
-    blocks, u8 = (cols + 31) // 32, rt.torch.uint8
+    blocks, u8 = (cols + 31) // 32, rt.u8
     a = Act8.__new__(Act8)
     a.codes, a.scales, a.cols = x.new_empty((n, blocks * 32), dtype=u8), x.new_empty((blocks, (n + 15) // 16 * 16), dtype=u8), cols
-    _on(rt, dev, "act8_pack", lib().agpt_b200_act8_pack, x.data_ptr(), ld, kind, a.codes.data_ptr(), a.scales.data_ptr(), n, cols)
+    _on(rt, dev, "act8_pack", rt.lib.agpt_b200_act8_pack, x.data_ptr(), ld, kind, a.codes.data_ptr(), a.scales.data_ptr(), n, cols)
     return a
 
 
 def act8_unpack(a: Act8):
     """The values of a checkpoint, float32 [n, cols]."""
     rt, n = _rt(), a.codes.shape[0]
-    out = a.codes.new_empty((n, a.cols), dtype=rt.torch.float32)
-    _on(rt, a.codes.get_device(), "act8_unpack", lib().agpt_b200_act8_unpack, a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr(), n, a.cols)
+    out = a.codes.new_empty((n, a.cols), dtype=rt.f32)
+    _on(rt, a.codes.get_device(), "act8_unpack", rt.lib.agpt_b200_act8_unpack, a.codes.data_ptr(), a.scales.data_ptr(), out.data_ptr(), n, a.cols)
     return out
 
 
@@ -1018,10 +1027,10 @@ def act8_relu_backward(grad, a: Act8, out=None):
     if cols != a.cols:
         raise AgptError(f"grad has {cols} columns, the activation {a.cols}")
     if out is None:
-        out = grad.new_empty((n, cols))
+        out = _new_rows(rt, grad, n, cols, ld)
     else:
         _rows_like(rt, out, "out", KV_F32, n, cols, dev, whole=True)
-    _on(rt, dev, "act8_relu_backward", lib().agpt_b200_act8_relu_backward, grad.data_ptr(), ld, a.codes.data_ptr(), out.data_ptr(), n, cols)
+    _on(rt, dev, "act8_relu_backward", rt.lib.agpt_b200_act8_relu_backward, grad.data_ptr(), ld, a.codes.data_ptr(), out.data_ptr(), n, cols)
     return out
 
 
@@ -1037,7 +1046,7 @@ def act8_weight_grad(a: Act8, grad, out=None, bias_grad: bool = True):
     else:
         _rows_like(rt, out, "out", KV_F32, a.cols, cols, dev, whole=True)
     db = grad.new_empty(cols) if bias_grad else None
-    L = lib()
+    L = rt.lib
     ws, need = _scratch_for(rt, grad, dev, "act8_weight_grad", L.agpt_b200_act8_weight_grad_workspace_bytes, n, a.cols, cols)
     _on(rt, dev, "act8_weight_grad", L.agpt_b200_act8_weight_grad, a.codes.data_ptr(), a.scales.data_ptr(), grad.data_ptr(), ld, n, a.cols, cols, out.data_ptr(),
         None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need)
