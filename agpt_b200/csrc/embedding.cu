@@ -11,11 +11,13 @@
 #include <cstdint>
 #include <mutex>
 #include <set>
+#include <type_traits>
 #include <utility>
 
 #include "../../include/agpt_b200.h"
 #include "internal.h"
 #include "pdl.cuh"
+#include "tc100.cuh"
 #include "vec.cuh"
 
 namespace {
@@ -210,6 +212,124 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
         }
         __syncwarp();
     }
+}
+
+// ---- the same in one cluster: up to CLUSTER_ROWS rows -----------------------------------------------------------------------------
+// Eight blocks hold all pairs in shared memory and exchange counts and pairs there, digits of eight bits a pass.  Three launches a pass of a few microseconds each are
+// most of a gradient of so few rows (5000 rows of 10,000 tokens, 256 columns: 19 us, 24 by six launches; 600 of 1400, 128: 15 and 19 by calls, 16 and 27).  From some
+// 60,000 rows on eight SMs take longer than all of them: 23 us of 65,537 rows, six launches 27.
+constexpr int CLUSTER = 8, CLUSTER_WARPS = 32, CLUSTER_THREADS = CLUSTER_WARPS * 32, CLUSTER_BITS = 8, CLUSTER_BINS = 1 << CLUSTER_BITS;
+constexpr int CLUSTER_CHUNK = 4 * 1024, CLUSTER_ROWS = CLUSTER * CLUSTER_CHUNK;
+constexpr int CLUSTER_SMEM = 2 * CLUSTER_CHUNK * 8 + (CLUSTER_WARPS + 3) * CLUSTER_BINS * 4;
+
+template <int SOURCE>
+__global__ void __launch_bounds__(CLUSTER_THREADS) cluster_sort_kernel(const void *__restrict__ source, int n, int chunk, uint32_t vocab, int passes, uint2 *__restrict__ out) {
+    pdl_wait();
+    pdl_next();
+    extern __shared__ __align__(16) uint32_t s_sort[];
+    uint2 *const pairs = reinterpret_cast<uint2 *>(s_sort);                        // [2][chunk]
+    uint32_t *const s_at = s_sort + 4 * chunk;                                     // counters, then places, of each warp [CLUSTER_WARPS][bins]
+    uint32_t *const s_total = s_at + CLUSTER_WARPS * CLUSTER_BINS, *const s_before = s_total + 2 * CLUSTER_BINS;      // digits of this block, by pass parity; of earlier blocks
+    __shared__ uint32_t s_warp[CLUSTER_WARPS];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, rank = blockIdx.x, own = chunk / CLUSTER_WARPS;
+    const int first = rank * chunk, rows = max(0, min(chunk, n - first)), i0 = w * own, i1 = min(i0 + own, rows);     // places of this block, and of this warp in it
+    uint32_t *const mine = s_at + w * CLUSTER_BINS;
+    // The first pass reads the tokens, the others the pairs in shared memory (known to the compiler: see above)
+    const auto one_pass = [&](auto from, int pass) {
+        constexpr bool TOKENS = decltype(from)::value;
+        const int shift = pass * CLUSTER_BITS;
+        const uint2 *const in = pairs + (pass & 1 ? 0 : chunk);                    // pass p writes half p & 1
+        const uint32_t into = tc::smem_u32(pairs + (pass & 1 ? chunk : 0));
+        const auto load = [&](int i) {
+            if constexpr (TOKENS) return pair_at<SOURCE>(source, first + i, vocab);
+            else return in[i];
+        };
+        for (int b = threadIdx.x; b < CLUSTER_WARPS * CLUSTER_BINS; b += CLUSTER_THREADS) s_at[b] = 0;
+        __syncthreads();
+        for (int i = i0 + lane; i < i1; i += 32 * 4) {
+            uint32_t key[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) key[k] = load(min(i + 32 * k, i1 - 1)).x;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + 32 * k < i1) atomicAdd(&mine[(key[k] >> shift) & (CLUSTER_BINS - 1)], 1u);
+        }
+        __syncthreads();
+        // a thread has a digit: its pairs in the warps before, its total here; then, with the other blocks' totals, its start
+        uint32_t *const total = s_total + (pass & 1) * CLUSTER_BINS;
+        if (threadIdx.x < CLUSTER_BINS) {
+            uint32_t at = 0;
+#pragma unroll 8
+            for (int k = 0; k < CLUSTER_WARPS; k++) {
+                const uint32_t x = s_at[k * CLUSTER_BINS + threadIdx.x];
+                s_at[k * CLUSTER_BINS + threadIdx.x] = at;
+                at += x;
+            }
+            total[threadIdx.x] = at;
+        }
+        tc::cluster_sync();                            // totals are there; every block has read the half that this pass writes
+        uint32_t all = 0, before = 0;
+        if (threadIdx.x < CLUSTER_BINS) {
+            const uint32_t here = tc::smem_u32(total + threadIdx.x);
+            uint32_t x[CLUSTER];
+#pragma unroll
+            for (int r = 0; r < CLUSTER; r++) x[r] = tc::peer_lds_u1(tc::peer_addr(here, r));
+#pragma unroll
+            for (int r = 0; r < CLUSTER; r++) {
+                all += x[r];
+                if (r < rank) before += x[r];
+            }
+        }
+        uint32_t run = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += x;
+        }
+        if (lane == 31) s_warp[w] = run;
+        __syncthreads();
+        if (threadIdx.x < CLUSTER_BINS) {
+            uint32_t at = run - all + before;
+            for (int k = 0; k < w; k++) at += s_warp[k];
+            s_before[threadIdx.x] = at;
+        }
+        __syncthreads();
+        for (int i = i0; i < i1; i += 32 * 4) {
+            uint2 p[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) p[r] = load(min(i + 32 * r + lane, i1 - 1));
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                if (i + 32 * r >= i1) break;
+                const bool live = i + 32 * r + lane < i1;
+                const uint32_t digit = (p[r].x >> shift) & (CLUSTER_BINS - 1);
+                uint32_t same = __ballot_sync(0xffffffffu, live);
+#pragma unroll
+                for (int k = 0; k < CLUSTER_BITS; k++) {
+                    const bool one = digit >> k & 1;
+                    const uint32_t ones = __ballot_sync(0xffffffffu, one);
+                    same &= one ? ones : ~ones;
+                }
+                uint32_t at = 0;
+                if (live) at = mine[digit] + __popc(same & ((1u << lane) - 1));
+                __syncwarp();
+                if (live) {
+                    if (lane == 31 - __clz(same)) mine[digit] = at + 1;      // the last of them
+                    const uint32_t to = s_before[digit] + at;
+                    if (pass + 1 == passes) out[to] = p[r];
+                    else {
+                        const uint32_t block = to / (uint32_t)chunk;
+                        tc::peer_sts_u2(tc::peer_addr(into + (to - block * chunk) * 8, block), p[r].x, p[r].y);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (pass + 1 < passes) tc::cluster_sync();     // pairs are there
+    };
+    one_pass(std::true_type(), 0);
+    for (int pass = 1; pass < passes; pass++) one_pass(std::false_type(), pass);
+    tc::cluster_sync();                                // no block leaves while another may read its totals
 }
 
 // ---- sums over the ordered rows ----------------------------------------------------------------------------------------------------
@@ -602,6 +722,18 @@ int sort_pass(const void *source, int64_t n, const Sizes &z, uint32_t vocab, int
     return AGPT_OK;
 }
 
+template <int SOURCE>
+int sort_in_cluster(const void *ids, int n, uint32_t vocab, uint2 *out, cudaStream_t st) {
+    const int own = ((n + CLUSTER * CLUSTER_WARPS - 1) / (CLUSTER * CLUSTER_WARPS) + 31) / 32 * 32, chunk = own * CLUSTER_WARPS;
+    int passes = 1;
+    while (passes * CLUSTER_BITS < 32 && (vocab >> (passes * CLUSTER_BITS)) > 0) passes++;
+    if (int rc = allow_smem(cluster_sort_kernel<SOURCE>, CLUSTER_SMEM)) return rc;
+    const size_t smem = (size_t)2 * chunk * 8 + (CLUSTER_WARPS + 3) * CLUSTER_BINS * 4;
+    const cudaError_t e = pdl_launch_clusters(cluster_sort_kernel<SOURCE>, CLUSTER, CLUSTER, CLUSTER_THREADS, smem, st, ids, n, chunk, vocab, passes, out);
+    if (e != cudaSuccess) return agpt_set_error(AGPT_E_CUDA, "embedding_grad_sorted: %s", cudaGetErrorString(e));
+    return AGPT_OK;
+}
+
 template <typename T, typename O, int VEC>
 int grad_sorted(const T *grad, int64_t ld, const void *ids, int wide, O *out, int64_t n, int d, uint32_t vocab, float scale, int accumulate, char *ws, cudaStream_t st) {
     const unsigned slices = (unsigned)((d + 32 * VEC - 1) / (32 * VEC));
@@ -611,20 +743,25 @@ int grad_sorted(const T *grad, int64_t ld, const void *ids, int wide, O *out, in
         return launch_status("embedding_grad_sorted");
     }
     const Sizes z = sizes_of(n, d, vocab);
-    uint2 *pairs[2] = {(uint2 *)(ws + z.at_pairs), (uint2 *)(ws + z.at_pairs) + n};
-    if (int rc = wide ? sort_pass<IDS64>(ids, n, z, vocab, 0, ws, pairs[0], st) : sort_pass<IDS32>(ids, n, z, vocab, 0, ws, pairs[0], st)) return rc;
-    for (int p = 1; p < z.passes; p++)
-        if (int rc = sort_pass<PAIRS>(pairs[(p - 1) & 1], n, z, vocab, p, ws, pairs[p & 1], st)) return rc;
-    const uint2 *order = pairs[(z.passes - 1) & 1];
+    const uint2 *order;
+    if (n <= CLUSTER_ROWS) {
+        if (int rc = wide ? sort_in_cluster<IDS64>(ids, (int)n, vocab, (uint2 *)(ws + z.at_pairs), st) : sort_in_cluster<IDS32>(ids, (int)n, vocab, (uint2 *)(ws + z.at_pairs), st)) return rc;
+        order = (uint2 *)(ws + z.at_pairs);
+    } else {
+        uint2 *pairs[2] = {(uint2 *)(ws + z.at_pairs), (uint2 *)(ws + z.at_pairs) + n};
+        if (int rc = wide ? sort_pass<IDS64>(ids, n, z, vocab, 0, ws, pairs[0], st) : sort_pass<IDS32>(ids, n, z, vocab, 0, ws, pairs[0], st)) return rc;
+        for (int p = 1; p < z.passes; p++)
+            if (int rc = sort_pass<PAIRS>(pairs[(p - 1) & 1], n, z, vocab, p, ws, pairs[p & 1], st)) return rc;
+        order = pairs[(z.passes - 1) & 1];
+    }
     float *head = (float *)(ws + z.at_head), *tail = (float *)(ws + z.at_tail);
     if (VEC > 1)
         if (int rc = allow_smem(sum_kernel<T, O, VEC>, SUM_WARPS * SUM_RING * 512)) return rc;
-    pdl_launch(sum_kernel<T, O, VEC>, dim3((unsigned)(z.blocks + fill), slices), SUM_WARPS * 32, VEC > 1 ? SUM_WARPS * SUM_RING * 512 : 0, st, grad, ld, order, n, d, vocab, z.run, z.blocks, scale, accumulate,
-               out, head, tail);
+    pdl_launch(sum_kernel<T, O, VEC>, dim3((unsigned)(z.blocks + fill), slices), SUM_WARPS * 32, VEC > 1 ? SUM_WARPS * SUM_RING * 512 : 0, st, grad, ld, order, n, d, vocab,
+               z.run, z.blocks, scale, accumulate, out, head, tail);
     if (z.blocks > 1)
-        pdl_launch(join_kernel<O>, dim3((unsigned)((z.blocks + 7) / 8), (unsigned)((d + 127) / 128)), 256, 0, st, order, n, d, vocab, (int64_t)SUM_WARPS * z.run, z.blocks, scale,
-                   accumulate,
-                   out, (const float *)head, (const float *)tail);
+        pdl_launch(join_kernel<O>, dim3((unsigned)((z.blocks + 7) / 8), (unsigned)((d + 127) / 128)), 256, 0, st, order, n, d, vocab, (int64_t)SUM_WARPS * z.run, z.blocks,
+                   scale, accumulate, out, (const float *)head, (const float *)tail);
     return launch_status("embedding_grad_sorted");
 }
 
@@ -648,11 +785,12 @@ int grad_by_output(const T *grad, int64_t ld, const void *ids, int wide, void *o
     constexpr int V = 16 / sizeof(T);
     // whole pieces: both the rows and, written by the same lanes, the table lie on 16-byte boundaries
     const bool whole = d % V == 0 && ld % V == 0 && vec::aligned(grad, 16) && vec::aligned(out, 16);
-    if (out_type == AGPT_KV_BF16)
-        return whole ? grad_sorted<T, bf16, V>(grad, ld, ids, wide, (bf16 *)out, n, d, vocab, scale, accumulate, ws, st)
-                     : grad_sorted<T, bf16, 1>(grad, ld, ids, wide, (bf16 *)out, n, d, vocab, scale, accumulate, ws, st);
-    return whole ? grad_sorted<T, float, V>(grad, ld, ids, wide, (float *)out, n, d, vocab, scale, accumulate, ws, st)
-                 : grad_sorted<T, float, 1>(grad, ld, ids, wide, (float *)out, n, d, vocab, scale, accumulate, ws, st);
+    const auto run = [&](auto *to) {
+        using O = std::remove_pointer_t<decltype(to)>;
+        return whole ? grad_sorted<T, O, V>(grad, ld, ids, wide, to, n, d, vocab, scale, accumulate, ws, st)
+                     : grad_sorted<T, O, 1>(grad, ld, ids, wide, to, n, d, vocab, scale, accumulate, ws, st);
+    };
+    return out_type == AGPT_KV_BF16 ? run((bf16 *)out) : run((float *)out);
 }
 
 int check_sizes(const char *who, int64_t n, int d, int64_t ld, int64_t vocab, int type) {

@@ -191,6 +191,12 @@ __device__ __forceinline__ ulonglong2 peer_lds_f4(uint32_t a) {
     asm volatile("ld.shared::cluster.v2.b64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ uint32_t peer_lds_u1(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void peer_sts_u2(uint32_t a, uint32_t x, uint32_t y) { asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory"); }
 __device__ __forceinline__ void peer_sts_f4(uint32_t a, f2 x, f2 y) { asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(a), "l"(x), "l"(y) : "memory"); }
 __device__ __forceinline__ float lds_f1(uint32_t a) {
     float v;

@@ -1,5 +1,5 @@
-"""embedding_lookup and embedding_grad_sorted against float64, at the borders of their ways: few rows in one launch and ordered rows, one to three passes of
-the sort, whole and odd pieces of a row, runs of a token inside a warp, across warps, across blocks and over all of them."""
+"""embedding_lookup and embedding_grad_sorted against float64, at the borders of their ways: few rows in one launch, rows ordered in one cluster and by many blocks, every number of
+passes of both sorts, whole and odd pieces of a row, runs of a token inside a warp, across warps, across blocks and over all of them."""
 import numpy as np
 import pytest
 
@@ -58,9 +58,10 @@ def _check_grad(torch, grad, ids, vocab, scale, out=None, **kw):
 @pytest.mark.parametrize("kind", ["zipf", "one", "distinct", "outside"])
 @pytest.mark.parametrize("n,vocab,d", [
     (0, 5, 8), (1, 1, 4), (2, 3, 1), (300, 1400, 384), (512, 40, 65), (513, 40, 65),          # both sides of the few-rows border
-    (1025, 1, 33), (4096, 2047, 128), (4097, 2048, 36),                                      # one pass of 11 bits, two passes
-    (5000, 70_000, 20), (3001, 5_000_000, 4),                                                # two and three passes
-    (20_011, 500, 132), (70_000, 3, 8),                                                      # runs of a token over many blocks
+    (1025, 1, 33), (1024, 255, 128), (4097, 256, 36), (5000, 70_000, 20), (3001, 20_000_000, 4),       # one cluster: passes of eight bits, one to four
+    (20_011, 500, 132), (32_768, 1000, 12),
+    (32_769, 2047, 12), (33_001, 2048, 20), (40_000, 70_000, 9), (33_333, 5_000_000, 4),     # many blocks: passes of up to eleven bits, one to three
+    (70_000, 3, 8),                                                                          # runs of a token over many blocks of the sums
 ])
 def test_gradient(cuda, kind, n, vocab, d):
     import torch
