@@ -3,9 +3,15 @@
 //   lookup     out[i] = scale * E[id_i], a zero row where id_i lies outside the vocabulary
 //   gradient   dE[t]  = scale * sum of g[i] over the rows i with id_i = t
 //
-// Both are bound by memory: a gradient reads n rows once.  The sums repeat bit for bit, without atomics on floating values: the rows
-// are ordered by token (a stable counting sort of (token, row) pairs, 8 bytes a row), pieces of the order are summed by warps, and what a
-// token has in several pieces is added in the order of the pieces.
+// The sums repeat bit for bit, without atomics on floating values: the rows are ordered by token (a stable counting sort of (token, row) pairs,
+// 8 bytes a row), pieces of the order are summed by warps, and what a token has in several pieces is added in the order of the pieces.  Up to 512 rows
+// need no order: the block of a token's first row looks for the others.
+//
+// Bound by memory where there are many columns: a gradient reads n rows once and writes the table once.  1.4M rows x 128 float32, 1000 tokens: lookup 108 us (6.7 TB/s
+// written), gradient 156 us, of which the sums 113 (6.4 TB/s read), the sort 28 and the joins 14; 65,537 x 1024 bfloat16, 50,021 tokens: 30 and 90 us (134 MB read, 205
+// written), sort 30.  Between a thousand and a hundred thousand rows the chain of short launches is what is left: 15 us at 600 x 128, 19 at 5000 x 256, 46 at 20,000 x 512
+// of 50,000 tokens (100 MB written).  Not kept: one cooperative launch with grid barriers for the whole sort (93 us where 90), pairs ordered in shared memory before they
+// are written (a pass of 1.4M rows 21 us where 17.5), pieces of eight bytes for narrow rows (52 us where 53 at 300,000 x 64).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -333,7 +339,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) cluster_sort_kernel(const voi
 }
 
 // ---- sums over the ordered rows ----------------------------------------------------------------------------------------------------
-// A warp has `run` places of the order and 32 * VEC columns, a block SUM_WARPS warps side by side.  Tokens that end where they began are
+// A warp has `run` places of the order (64, fewer while there are less than eight blocks an SM) and 32 * VEC columns, a block SUM_WARPS warps side by side.  Tokens that end where they began are
 // written; the warps' first and last sums meet in shared memory; what a block has of a token that began before it goes to head[block], of
 // one that goes on behind it to tail[block], and join_kernel adds tail and heads in order.
 constexpr int SUM_WARPS = 8, SUM_RING = 8, FILL_TOKENS = 64;
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restr
         };
         if constexpr (VEC > 1) {
             // Rows come by asynchronous copies into a ring that only the copying lane reads: SUM_RING rows of every warp are on their way without a register each.
-            // (Eight rows in registers at a time left the loads waiting for the sums: 142 us at 1.4M x 128, two batches of four 150 to 175, this 119.)
+            // (Eight rows in registers at a time left the loads waiting for the sums: 142 us of this kernel at 1.4M x 128, two batches of four 150 and more, this 113.)
             const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_rows) + (w * SUM_RING * 32 + lane) * 16;
             const auto fetch = [&](int k) {
                 if (k < live) {
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ ord
 
 // ---- few rows: one launch, no order -------------------------------------------------------------------------------------------------
 // Every block reads all tokens; the block of a token's first row adds its rows, a run of the rows per warp; blocks behind fill absent tokens.
-constexpr int FEW_ROWS = 512;
+constexpr int FEW_ROWS = 512;      // 5 us at 301 rows x 384, 1400 tokens; every block looks at all rows
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(256) few_rows_kernel(const T *__restrict__ grad, int64_t ld, const void *__restrict__ ids, int wide, int n, int d, uint32_t vocab,
                                                         float scale, int accumulate, O *__restrict__ out) {
