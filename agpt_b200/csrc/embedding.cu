@@ -408,12 +408,14 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restr
     const int64_t p0 = ((int64_t)blockIdx.x * SUM_WARPS + w) * run, p1 = min(p0 + run, n);
     if (p0 < n) {
         const uint2 none = make_uint2(vocab, 0);
-        const uint2 near = p0 + lane < p1 ? __ldg(order + p0 + lane) : none, far = p0 + 32 + lane < p1 ? __ldg(order + p0 + 32 + lane) : none;      // at most 64 places
+        uint2 near = __ldg(order + min(p0 + lane, p1 - 1)), far = __ldg(order + min(p0 + 32 + lane, p1 - 1));      // at most 64 places
+        if (p0 + lane >= p1) near = none;
+        if (p0 + 32 + lane >= p1) far = none;
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; i++) acc[i] = 0.f;
-        const uint32_t first = __ldg(&order[p0].x), last = __ldg(&order[p1 - 1].x);
-        const bool in = p0 > 0 && __ldg(&order[p0 - 1].x) == first, goes_on = p1 < n && __ldg(&order[p1].x) == last;
+        const uint32_t first = __ldg(&order[p0].x), last = __ldg(&order[p1 - 1].x), ahead = __ldg(&order[max(p0 - 1, (int64_t)0)].x), behind = __ldg(&order[min(p1, n - 1)].x);
+        const bool in = p0 > 0 && ahead == first, goes_on = p1 < n && behind == last;
         uint32_t cur = first;
         bool begun_before = in;
         const int live = (int)(p1 - p0);
@@ -550,9 +552,10 @@ __global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ ord
     int64_t heads = 0;
     uint32_t key = vocab;
     if (b < blocks && p1 < n) {
+        // four loads at once
         key = __ldg(&order[p1 - 1].x);
-        const bool goes_on = key < vocab && __ldg(&order[p1].x) == key;
-        const bool before = p0 > 0 && __ldg(&order[p0].x) == key && __ldg(&order[p0 - 1].x) == key;
+        const uint32_t behind = __ldg(&order[p1].x), first = __ldg(&order[p0].x), ahead = __ldg(&order[max(p0 - 1, (int64_t)0)].x);
+        const bool goes_on = key < vocab && behind == key, before = p0 > 0 && first == key && ahead == key;
         if (goes_on && !before) {
             // blocks behind that begin with the token: they are the first ones, so 32 are asked at a time, near ones first, then by 32nds of what is left
             int64_t low = 1, high = blocks - b;                        // `low` of them are known to, from `high` on none does
