@@ -407,10 +407,7 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restr
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * COLS + lane * VEC;
     const int64_t p0 = ((int64_t)blockIdx.x * SUM_WARPS + w) * run, p1 = min(p0 + run, n);
     if (p0 < n) {
-        const uint2 none = make_uint2(vocab, 0);
-        uint2 near = __ldg(order + min(p0 + lane, p1 - 1)), far = __ldg(order + min(p0 + 32 + lane, p1 - 1));      // at most 64 places
-        if (p0 + lane >= p1) near = none;
-        if (p0 + 32 + lane >= p1) far = none;
+        const uint2 near = __ldg(order + min(p0 + lane, p1 - 1)), far = __ldg(order + min(p0 + 32 + lane, p1 - 1));      // at most 64 places
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; i++) acc[i] = 0.f;
@@ -418,24 +415,21 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restr
         const bool in = p0 > 0 && ahead == first, goes_on = p1 < n && behind == last;
         uint32_t cur = first;
         bool begun_before = in;
-        const int live = (int)(p1 - p0);
-        const auto pair = [&](int k) {
-            const uint2 x = k < 32 ? near : far;
-            return make_uint2(__shfl_sync(0xffffffffu, x.x, k & 31), __shfl_sync(0xffffffffu, x.y, k & 31));
-        };
-        const auto add = [&](uint32_t key, const float (&v)[VEC]) {
-            if (key != cur) {
-                if (begun_before) {
+        // rows outside the vocabulary are last: a warp that begins with one has nothing to add, and sums of theirs are written nowhere
+        const int live = first < vocab ? (int)(p1 - p0) : 0;
+        // bit k: place k has another token than place k - 1
+        const uint32_t left = __shfl_up_sync(0xffffffffu, near.x, 1), left2 = __shfl_up_sync(0xffffffffu, far.x, 1), middle = __shfl_sync(0xffffffffu, near.x, 31);
+        const uint64_t change = (uint64_t)__ballot_sync(0xffffffffu, far.x != (lane ? left2 : middle)) << 32 | __ballot_sync(0xffffffffu, lane && near.x != left);
+        const auto row_at = [&](int k) { return __shfl_sync(0xffffffffu, k < 32 ? near.y : far.y, k & 31); };
+        const auto next_token = [&](int k) {
+            if (begun_before) {
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) s_part[w][0][lane * VEC + i] = acc[i];
-                } else if (cur < vocab && c < d) write_row<O, VEC>(out, (int64_t)cur * d + c, acc, scale, accumulate);
-                cur = key;
-                begun_before = false;
+                for (int i = 0; i < VEC; i++) s_part[w][0][lane * VEC + i] = acc[i];
+            } else if (cur < vocab && c < d) write_row<O, VEC>(out, (int64_t)cur * d + c, acc, scale, accumulate);
+            cur = __shfl_sync(0xffffffffu, k < 32 ? near.x : far.x, k & 31);
+            begun_before = false;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) acc[i] = 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; i++) acc[i] += v[i];
+            for (int i = 0; i < VEC; i++) acc[i] = 0.f;
         };
         if constexpr (VEC > 1) {
             // Rows come by asynchronous copies into a ring that only the copying lane reads: SUM_RING rows of every warp are on their way without a register each.
@@ -443,39 +437,42 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restr
             const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_rows) + (w * SUM_RING * 32 + lane) * 16;
             const auto fetch = [&](int k) {
                 if (k < live) {
-                    const uint2 x = pair(k);
-                    if (x.x < vocab && c < d)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (k % SUM_RING) * 512), "l"(grad + (int64_t)x.y * ld + c) : "memory");
+                    const T *from = grad + (int64_t)row_at(k) * ld + c;
+                    if (c < d) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (k % SUM_RING) * 512), "l"(from) : "memory");
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
 #pragma unroll
             for (int k = 0; k < SUM_RING - 1; k++) fetch(k);
-            for (int k = 0; k < live; k++) {
-                fetch(k + SUM_RING - 1);
-                asm volatile("cp.async.wait_group %0;" ::"n"(SUM_RING - 1) : "memory");
-                vec::Piece<T, VEC> piece;
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(piece.w[0]), "=r"(piece.w[1]), "=r"(piece.w[2]), "=r"(piece.w[3]) : "r"(ring + (k % SUM_RING) * 512) : "memory");
-                float v[VEC];
-                piece.values(v);
-                add(pair(k).x, v);
-            }
+            for (int k0 = 0; k0 < live; k0 += SUM_RING)
+#pragma unroll
+                for (int u = 0; u < SUM_RING; u++) {
+                    const int k = k0 + u;
+                    if (k >= live) break;
+                    fetch(k + SUM_RING - 1);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(SUM_RING - 1) : "memory");
+                    vec::Piece<T, VEC> piece;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(piece.w[0]), "=r"(piece.w[1]), "=r"(piece.w[2]), "=r"(piece.w[3]) : "r"(ring + u * 512) : "memory");
+                    float v[VEC];
+                    piece.values(v);
+                    if (change >> k & 1) next_token(k);
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) acc[i] += v[i];
+                }
         } else {
             constexpr int U = 8;
             for (int k0 = 0; k0 < live; k0 += U) {
                 vec::Piece<T, VEC> piece[U];
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const uint2 x = pair(k0 + u);
-                    piece[u].fetch(grad + (int64_t)x.y * ld + c, k0 + u < live && x.x < vocab && c < d);
-                }
+                for (int u = 0; u < U; u++) piece[u].fetch(grad + (int64_t)row_at(k0 + u) * ld + c, k0 + u < live && c < d);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const uint32_t key = pair(k0 + u).x;
                     if (k0 + u >= live) break;
                     float v[VEC];
                     piece[u].values(v);
-                    add(key, v);
+                    if (change >> (k0 + u) & 1) next_token(k0 + u);
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) acc[i] += v[i];
                 }
             }
         }
