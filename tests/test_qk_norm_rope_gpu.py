@@ -81,6 +81,35 @@ def test_outputs_of_another_type_and_in_place(cuda, hd):
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(x[:, 2 * h * hd:], v)              # and nothing beside them
 
 
+@pytest.mark.parametrize("hd,pad", [(32, 8), (32, 3), (40, 2), (128, 16)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("out_dtype", ["f32", "bf16"])
+def test_outputs_in_columns_of_wider_rows(cuda, hd, pad, dtype, out_dtype):
+    """Outputs of both types written into column ranges, on and off 16-byte boundaries, leave what lies beside them."""
+    import torch
+    n, hq, hk = 29, 5, 2
+    t = torch.bfloat16 if out_dtype == "bf16" else torch.float32
+    q, k = _rows(torch, cuda, n, hq * hd, dtype, "whole", 1), _rows(torch, cuda, n, hk * hd, dtype, "whole", 2)
+    cos, sin = [torch.from_numpy(x).to(cuda) for x in F.rope_table(16, hd)]
+    pos = torch.randint(0, 16, (n,), device=cuda, dtype=torch.int32)
+    wide = [torch.full((n, h * hd + 2 * pad), 7.0, device=cuda, dtype=t) for h in (hq, hk)]
+    views = [w[:, pad:w.shape[1] - pad] for w in wide]
+    A.qk_norm_rope(q, k, None, None, pos, cos, sin, q_out=views[0], k_out=views[1])
+    for got, w, x in zip(views, wide, (q, k)):
+        _close(got, *F.norm_rope(_np(x), None, pos.cpu().numpy(), cos.cpu().numpy(), sin.cpu().numpy(), 1e-6), out_dtype)
+        assert bool((w[:, :pad] == 7).all()) and bool((w[:, -pad:] == 7).all())
+    if dtype == out_dtype:
+        dy = [_rows(torch, cuda, n, h * hd, "f32", "odd", 3) for h in (hq, hk)]
+        A.qk_norm_rope_backward(*dy, q, k, None, None, pos, cos, sin, q_out=views[0], k_out=views[1])
+        want = A.qk_norm_rope_backward(*dy, q, k, None, None, pos, cos, sin)
+        for got, w, x, d in zip(views, wide, (q, k), dy):
+            _close(got, *F.norm_rope_backward(_np(d), _np(x), None, pos.cpu().numpy(), cos.cpu().numpy(), sin.cpu().numpy(), 1e-6)[:2], out_dtype)
+            assert bool((w[:, :pad] == 7).all()) and bool((w[:, -pad:] == 7).all())
+        assert want[0].dtype == q.dtype
+    y = A.qk_norm_rope(q, k, None, None, pos, cos, sin, k_dtype=t)
+    assert y[0].dtype == q.dtype and y[1].dtype == t
+
+
 def test_zero_rows_positions_outside_the_tables_and_infinities(cuda):
     import torch
     hd, n = 32, 6
