@@ -206,10 +206,10 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // through shared memory, so that a split of G serves all of them.  TMA brings the raw rows; rows of G that it cannot take (off 16-byte boundaries) are copied four
 // bytes at a time by the threads that convert them.  Blocks own (G tile, X columns, slice of the rows); slices are added in order.
 //
-// 400k rows: 512 kept columns, G of 128: 136 us (1150 TFLOP/s of MMAs); 128 kept, G of 512: 175 us (4.9 TB/s); error against float64 3e-7.  What bounds it is shared
+// 400k rows: 512 kept columns, G of 128: 136 us (1150 TFLOP/s of MMAs); 128 kept, G of 512: 171 us (5.1 TB/s); error against float64 3e-7.  What bounds it is shared
 // memory: per 64 rows of 128 x 256 the raw rows in and out, the planes and the MMAs' reads of them, each plane of G against the same codes, move 224 KB, 1750 clocks at
 // 128 bytes, where the MMAs take 1536 and the memory 1100.  On the way here: accumulators drained every 64 rows by eight columns at a time 245 and 411 us, by TMA
-// and 16 columns 209 and 289, every 128 rows 155 and 222 (error 1e-7 to 3e-7), eight warps on X 157 and 178, both groups on each accumulator 139 and 177.  Slower: stages
+// and 16 columns 209 and 289, every 128 rows 155 and 222 (error 1e-7 to 3e-7), eight warps on X 157 and 178, both groups on each accumulator 139 and 177, all threads on 128 columns of X 136 and 171.  Slower: stages
 // of 32 rows (143 and 206), eight warps on G (146 and 207).
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
 constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, eight on the accumulators
@@ -397,13 +397,14 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
         if (P.col_part && x0 == 0 && live) P.col_part[(int64_t)slice * P.cols + col] = csum;
     } else if (warp < 16) {
         regs_dec<REG_X>();
-        // ---------------- X: a thread has 16 columns of four rows ----------------
-        const int t = tid - 256, piece = t & 15, row4 = (t >> 4) * 4;
+        // ---------------- X: a thread has 16 columns of four rows; of two where the block has up to 128 columns, since half of the
+        // threads would have none otherwise: 400k rows of 128 by 512 take 171 us against 180 ----------------
+        const int narrow = P.x_cols <= ACC_COLS, t = tid - 256, piece = t & (narrow ? 7 : 15), rows = narrow ? 2 : 4;
+        const int row = (t >> (narrow ? 3 : 4)) * rows;
         const bool live = piece * 16 < P.x_cols;
-        const uint32_t raw = base + OFF_X + row4 * P.x_cols + piece * 16, raw_s = base + OFF_S + (piece >> 1) * WG_ROWS + row4;
+        const uint32_t raw = base + OFF_X + row * P.x_cols + piece * 16, raw_s = base + OFF_S + (piece >> 1) * WG_ROWS + (row & ~3);
         // place of the first stored half piece: eight neighbouring lanes write eight different 16-byte chunks of a row
-        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row4 * 128;
-        const uint32_t even = row4 & 4, at = (piece & 3) * 2 + swap, at2 = at ^ 1;
+        const uint32_t swap = (piece >> 2) & 1, put = base + OFF_P + ((piece >> 2) << 13) + row * 128, at = (piece & 3) * 2 + swap, at2 = at ^ 1, row7 = row & 7;
         uint32_t i = 0, xp = 0;
         int slot = 0;
         for (int64_t rb = rb0; rb < rb1; rb++, i++) {
@@ -413,15 +414,17 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
                 uint32_t sc;
                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(sc) : "r"(raw_s + slot * RAW_S));
                 if (rb == P.row_blocks - 1) {                          // scales behind the last row may hold anything
-                    const int64_t rows = P.n - (rb * WG_ROWS + row4);
-                    const uint32_t past = rows >= 4 ? 0 : rows <= 0 ? 0xffffffffu : 0xffffffffu << (8 * (int)rows);
+                    const int64_t left = P.n - (rb * WG_ROWS + (row & ~3));
+                    const uint32_t past = left >= 4 ? 0 : left <= 0 ? 0xffffffffu : 0xffffffffu << (8 * (int)left);
                     sc = (sc & ~past) | (0x7f7f7f7fu & past);
                 }
+                sc >>= 8 * (row & 3);
                 // 2^(scale - 7) is a bfloat16 up to 134; above, 2^127 and a second factor (255: NaN)
                 const bool large = __vcmpgtu4(sc, 0x86868686u);
                 const uint32_t from = raw + slot * RAW_X, to = put + st * PLANE;
 #pragma unroll
-                for (uint32_t k = 0; k < 4; k++) {
+                for (int k = 0; k < 4; k++) {
+                    if (k >= rows) break;
                     uint32_t w[4], a[4], b[4];
                     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from + k * P.x_cols + swap * 8));
                     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "r"(from + k * P.x_cols + 8 - swap * 8));
@@ -436,8 +439,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
 #pragma unroll
                         for (int i = 0; i < 4; i++) { a[i] = mul_bf16x2(a[i], two); b[i] = mul_bf16x2(b[i], two); }
                     }
-                    sts_u4(to + k * 128 + (at ^ (even | k)) * 16, a);
-                    sts_u4(to + k * 128 + (at2 ^ (even | k)) * 16, b);
+                    sts_u4(to + k * 128 + (at ^ (row7 + k)) * 16, a);
+                    sts_u4(to + k * 128 + (at2 ^ (row7 + k)) * 16, b);
                 }
             }
             fence_async_smem();
