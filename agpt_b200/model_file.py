@@ -7,6 +7,7 @@ wo.b, ln1.gamma, ln1.beta, l1.w, l1.b, l2.w, l2.b, ln2.gamma, ln2.beta; final ga
 """
 from __future__ import annotations
 
+import os
 import struct
 from dataclasses import dataclass, field
 
@@ -101,6 +102,15 @@ def save_gains(path: str, gains) -> None:
             a = np.ascontiguousarray(a, dtype="<f4")
             f.write(struct.pack("<2i", 1, a.size))
             f.write(a.tobytes())
+
+
+def save_with_gains(path: str, m: Model, gains) -> None:
+    """The model file and, beside it, its gains file.  Without gains, one that an earlier model left there goes: it would be read as this model's."""
+    save(path, m)
+    if gains:
+        save_gains(path + GAINS_SUFFIX, gains)
+    elif os.path.exists(path + GAINS_SUFFIX):
+        os.remove(path + GAINS_SUFFIX)
 
 
 def gain_names(n_layers: int):

@@ -919,11 +919,6 @@ def main(argv=None):
     n_sub = int((trie.parent[1:] == 0).sum())
     # optimizer steps per epoch, as the reference counts them for its schedule (src/cuda/agpt_train.cu:5100-5117)
     per_epoch = args.lightning_steps if lightning else (len(groups) if (args.no_accumulate and world == 1) else 1)
-    def save_model(path):
-        MF.save(path, model.to_model_file())
-        if model.qk_norm:
-            MF.save_gains(path + MF.GAINS_SUFFIX, model.qk_gains())
-
     if args.lr_schedule != "constant":
         opt.schedule = (args.lr_schedule, max(per_epoch * args.epochs, 1), args.warmup_epochs * per_epoch)
     save = args.save or args.model
@@ -945,9 +940,9 @@ def main(argv=None):
             print(f"Epoch {ep}: loss={ls / max(nq, 1):.6f}  ({time.time() - t0:.2f} sec, {units} subtrees, {chunks} chunks, {nq} nodes)",
                   flush=True)
             if args.save_every and ep % args.save_every == 0:
-                save_model(f"{save}.ep{ep}")
+                MF.save_with_gains(f"{save}.ep{ep}", model.to_model_file(), model.qk_gains())
     if rank == 0:
-        save_model(save)
+        MF.save_with_gains(save, model.to_model_file(), model.qk_gains())
     if world > 1:
         dist.destroy_process_group()
 
