@@ -209,8 +209,8 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // 400k rows: 512 kept columns, G of 128: 136 us (1150 TFLOP/s of MMAs); 128 kept, G of 512: 171 us (5.1 TB/s); error against float64 3e-7.  What bounds it is shared
 // memory: per 64 rows of 128 x 256 the raw rows in and out, the planes and the MMAs' reads of them, each plane of G against the same codes, move 224 KB, 1750 clocks at
 // 128 bytes, where the MMAs take 1536 and the memory 1100.  On the way here: accumulators drained every 64 rows by eight columns at a time 245 and 411 us, by TMA
-// and 16 columns 209 and 289, every 128 rows 155 and 222 (error 1e-7 to 3e-7), eight warps on X 157 and 178, both groups on each accumulator 139 and 177, all threads on 128 columns of X 136 and 171.  Slower: stages
-// of 32 rows (143 and 206), eight warps on G (146 and 207).
+// and 16 columns 209 and 289, every 128 rows 155 and 222 (error 1e-7 to 3e-7), eight warps on X 157 and 178, both groups on each accumulator 139 and 177, all threads on
+// 128 columns of X 136 and 171.  Slower: stages of 32 rows (143 and 206), eight warps on G (146 and 207).
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
 constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, eight on the accumulators
 constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 8 * WG_ROWS, PLANE = WG_ROWS * WG_X * 2;

@@ -29,7 +29,6 @@ using tc::f2_add; using tc::f2_fma; using tc::f2_get; using tc::f2_mul; using tc
 // Blocks of the backward on an SM by the bytes of an element of x: in float32 four (674 us at 1.4M x 8 x 32, three 711), in bfloat16, with eight columns a lane, three
 constexpr int back_blocks(int bytes) { return bytes == 4 ? 4 : 3; }
 
-
 struct Rows {                          // queries or keys: heads * head_dim columns, rows ld elements apart
     const void *x, *dy;
     void *out;                         // y, or dx
