@@ -936,7 +936,8 @@ def qk_norm_rope(q, k, q_gain, k_gain, pos, cos, sin, eps: float = 1e-6, k_dtype
 
 def qk_norm_rope_backward(dq, dk, q, k, q_gain, k_gain, pos, cos, sin, dq_gain=None, dk_gain=None, eps: float = 1e-6, q_out=None, k_out=None):
     """Gradients of qk_norm_rope with respect to q and k (of their type), from those of its outputs (dq, dk: both float32 or both bfloat16) and
-    its inputs.  dq_gain, dk_gain [head_dim] float32 are accumulated into (None: not wanted).  q_out and k_out may be dq and dk."""
+    its inputs.  dq_gain, dk_gain [head_dim] float32 are accumulated into (None: not wanted; one tensor for both, of a shared gain, takes both sums).
+    q_out and k_out may be dq and dk."""
     rt = _rt()
     kind, n, qc, q_ld, dev = _rows(rt, q, "q")
     kc = k.shape[-1]

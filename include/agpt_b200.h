@@ -402,7 +402,8 @@ int64_t agpt_b200_embedding_grad_sorted_workspace_bytes(int64_t n, int d_model, 
  * that keys can go straight into a bfloat16 store; an output may be its input where types and strides are equal.  Gains [head_dim] float32, NULL: ones.
  * eps must be above 0.
  * Backward: from dq, dk of grad_type and the forward's inputs, the gradients with respect to q and k (of their type; may be written over dq and dk of that type
- * and stride).  Gain gradients [head_dim] float32 are accumulated into in a fixed order (NULL: not wanted; with both NULL no workspace is needed). */
+ * and stride).  Gain gradients [head_dim] float32 are accumulated into in a fixed order (NULL: not wanted; with both NULL no workspace is needed); one tensor for
+ * both, where queries and keys share their gain, takes the queries' sum and then the keys'. */
 int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void *d_k, int64_t k_ld, int type, const float *d_q_gain, const float *d_k_gain,
                            const int32_t *d_pos, const float *d_cos, const float *d_sin, int n_pos, int64_t n, int q_heads, int k_heads,
                            int head_dim, float eps, void *d_q_out, int64_t q_out_ld, int q_out_type, void *d_k_out, int64_t k_out_ld,
