@@ -247,6 +247,14 @@ template <int HIGH> __device__ __forceinline__ uint32_t expand2(uint32_t w, uint
     asm("prmt.b32 %0, %1, 0, %2;" : "=r"(b) : "r"(w), "n"(HIGH ? 0xb3a2 : 0x9180));
     return mul_bf16x2(b << 4 & 0x87f087f0u, f);
 }
+// Codes of magnitude 0x7f are e4m3's NaN (pack writes them with scale byte 255 alone, a caller's own may have any).  Bit 7 of a byte: its code is one.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }
+// a pair of factors, NaN for the codes that are
+template <int HIGH> __device__ __forceinline__ uint32_t or_nan2(uint32_t w, uint32_t factors) {
+    uint32_t m;                                                        // each byte's bit 7 over its half of the word
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(m) : "r"(nan_codes(w)), "n"(HIGH ? 0xbbaa : 0x9988));
+    return factors | (m & 0x7fc07fc0u);
+}
 
 template <bool TMA_G>
 __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_constant__ WeightGrad P) {
@@ -419,7 +427,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
                     sc = (sc & ~past) | (0x7f7f7f7fu & past);
                 }
                 sc >>= 8 * (row & 3);
-                // 2^(scale - 7) is a bfloat16 up to 134; above, 2^127 and a second factor (255: NaN)
+                // 2^(scale - 7) is a bfloat16 up to 134; above, 2^127 and a second factor (255: NaN), which NaN codes take as well
                 const bool large = __vcmpgtu4(sc, 0x86868686u);
                 const uint32_t from = raw + slot * RAW_X, to = put + st * PLANE;
 #pragma unroll
@@ -434,10 +442,13 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
                         a[2 * i] = expand2<0>(w[i], f); a[2 * i + 1] = expand2<1>(w[i], f);
                         b[2 * i] = expand2<0>(w[2 + i], f); b[2 * i + 1] = expand2<1>(w[2 + i], f);
                     }
-                    if (large) {
+                    if (large || (nan_codes(w[0]) | nan_codes(w[1]) | nan_codes(w[2]) | nan_codes(w[3])) & 0x80808080u) {
                         const uint32_t two = s == 255 ? 0x7fc07fc0u : s > 134 ? (s - 7) * 0x00800080u : 0x3f803f80u;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) { a[i] = mul_bf16x2(a[i], two); b[i] = mul_bf16x2(b[i], two); }
+                        for (int i = 0; i < 2; i++) {
+                            a[2 * i] = mul_bf16x2(a[2 * i], or_nan2<0>(w[i], two)); a[2 * i + 1] = mul_bf16x2(a[2 * i + 1], or_nan2<1>(w[i], two));
+                            b[2 * i] = mul_bf16x2(b[2 * i], or_nan2<0>(w[2 + i], two)); b[2 * i + 1] = mul_bf16x2(b[2 * i + 1], or_nan2<1>(w[2 + i], two));
+                        }
                     }
                     sts_u4(to + k * 128 + (at ^ (row7 + k)) * 16, a);
                     sts_u4(to + k * 128 + (at2 ^ (row7 + k)) * 16, b);
