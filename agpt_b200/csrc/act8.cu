@@ -256,6 +256,35 @@ template <int HIGH> __device__ __forceinline__ uint32_t or_nan2(uint32_t w, uint
     return factors | (m & 0x7fc07fc0u);
 }
 
+// Two floats as the packed sums of three bfloat16 each: eight bits of the fraction are cut off at a time, which is exact for every finite value (a first part that is
+// rounded instead, as in tc::split3, is infinity from 0x7f7f8000 on, and its rest infinity the other way).
+__device__ __forceinline__ void cut3(tc::f2 xy, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+    using namespace tc;
+    const f2 minus_one = 0xbf800000bf800000ull;
+    uint32_t a, b;
+    f2_unpack(xy, a, b);
+    p0 = __byte_perm(a, b, 0x7632);
+    const f2 r = f2_fma(f2_pack(a & 0xffff0000u, b & 0xffff0000u), minus_one, xy);
+    f2_unpack(r, a, b);
+    p1 = __byte_perm(a, b, 0x7632);
+    f2_unpack(f2_fma(f2_pack(a & 0xffff0000u, b & 0xffff0000u), minus_one, r), a, b);
+    p2 = __byte_perm(a, b, 0x7632);
+}
+// The same where infinities and NaN may be among them: these are their first part alone, so that their products are infinities and NaN as those of any float are.
+__device__ __forceinline__ void cut3_any(tc::f2 xy, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+    using namespace tc;
+    cut3(xy, p0, p1, p2);
+    uint32_t a, b;
+    f2_unpack(xy, a, b);
+    const bool odd_a = (a & 0x7f800000u) == 0x7f800000u, odd_b = (b & 0x7f800000u) == 0x7f800000u;
+    const uint32_t keep = (odd_a ? 0 : 0xffffu) | (odd_b ? 0 : 0xffff0000u);
+    p1 &= keep;
+    p2 &= keep;
+    // NaN whose fraction was cut off
+    if (odd_a && a & 0x7fffffu) p0 |= 0x7fc0u;
+    if (odd_b && b & 0x7fffffu) p0 |= 0x7fc00000u;
+}
+
 template <bool TMA_G>
 __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_constant__ WeightGrad P) {
     using namespace tc;
@@ -388,14 +417,27 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
                 for (int k = 0; k < 16; k += 2) {
                     const f2 v = f2_pack(lds_f1(from + (k0 + k) * 512), lds_f1(from + (k0 + k + 1) * 512));
                     bsum = f2_add(bsum, v);
-                    split3(v, p[0][k >> 1], p[1][k >> 1], p[2][k >> 1]);
+                    cut3(v, p[0][k >> 1], p[1][k >> 1], p[2][k >> 1]);
                 }
 #pragma unroll
                 for (int q = 0; q < 3; q++) tmem_st8(dst + q * 32 + (k0 >> 1), p[q]);
             }
             const float2 b2 = f2_get(bsum);
-            csum += b2.x + b2.y;
+            const float block_sum = b2.x + b2.y;
+            csum += block_sum;
             tmem_wait_st();
+            // the sum is finite, or there are infinities or NaN among the values (or it went beyond the largest float): they are cut again with an eye to these
+            if (__any_sync(0xffffffffu, (__float_as_uint(block_sum) & 0x7f800000u) == 0x7f800000u)) {
+#pragma unroll 1
+                for (int k0 = 0; k0 < WG_ROWS; k0 += 16) {
+                    uint32_t p[3][8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) cut3_any(f2_pack(lds_f1(from + (k0 + 2 * k) * 512), lds_f1(from + (k0 + 2 * k + 1) * 512)), p[0][k], p[1][k], p[2][k]);
+#pragma unroll
+                    for (int q = 0; q < 3; q++) tmem_st8(dst + q * 32 + (k0 >> 1), p[q]);
+                }
+                tmem_wait_st();
+            }
             fence_before();
             __syncwarp();
             if (lane == 0) { if (TMA_G) mbar_arrive(gE + 8 * slot); mbar_arrive(tF + 8 * st); }

@@ -1,4 +1,4 @@
-"""What a checkpoint of unusual codes stands for is the same in every call over it."""
+"""What a checkpoint of unusual codes and a gradient of unusual numbers stand for is the same in every call: NaN codes, infinities, what lies next to the largest float."""
 import numpy as np
 import pytest
 
@@ -49,3 +49,25 @@ def test_nan_codes_are_nan_in_the_weight_gradient(cuda, n, m, cols):
     _same(db, sums, bound_b)
     mask = A.act8_unpack(a) > 0
     assert torch.equal(A.act8_relu_backward(torch.ones(n, m, device=cuda), a) > 0, mask)
+
+
+@pytest.mark.parametrize("n,m,cols,pad", [(5, 33, 8, 0), (150, 130, 64, 0), (150, 100, 61, 1), (300, 260, 129, 3)])
+def test_gradients_of_infinity_and_next_to_the_largest_float(cuda, n, m, cols, pad):
+    import torch
+    rng = np.random.default_rng(m)
+    x = (2.0 ** -20 * (1 + rng.random((n, m)))).astype(np.float32) * rng.choice(np.array([-1, 1], np.float32), (n, m))
+    x[rng.random((n, m)) < 0.05] = 0
+    g = rng.standard_normal((n, cols + 2 * pad)).astype(np.float32)
+    top = np.float32(3.4028235e38)
+    edge = np.uint32(0x7f7f8000).view(np.float32)                 # the first number that bfloat16 rounds to infinity
+    put = [np.inf, -np.inf, top, -top, edge, np.nextafter(edge, np.float32(0)), np.uint32(0x7f7f0001).view(np.float32), -np.uint32(0x7f7fabcd).view(np.float32)]
+    for k, v in enumerate(put):
+        g[rng.integers(n), pad + k % cols] = v
+    if cols > len(put) + 2:                                       # infinities of both signs, and NaN, in a column
+        g[0, pad + len(put)], g[n - 1, pad + len(put)], g[n // 2, pad + len(put) + 1] = np.inf, -np.inf, np.nan
+    a, grad = A.act8_pack(torch.from_numpy(x).to(cuda)), torch.from_numpy(g).to(cuda)[:, pad:pad + cols]
+    want, sums, bound, bound_b = _product(a, grad)
+    assert np.isinf(want).any() and np.isnan(want).any() and np.isfinite(want[:, 2:8]).all()
+    dw, db = A.act8_weight_grad(a, grad)
+    _same(dw, want, bound)
+    _same(db, sums, bound_b)
