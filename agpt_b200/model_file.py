@@ -104,13 +104,40 @@ def save_gains(path: str, gains) -> None:
             f.write(a.tobytes())
 
 
-def save_with_gains(path: str, m: Model, gains) -> None:
-    """The model file and, beside it, its gains file.  Without gains, one that an earlier model left there goes: it would be read as this model's."""
+# The factor on the embedding, which is part of the function that the weights were trained for: a file beside the model, u32 magic, f64 factor; no file: 1.
+SCALE_MAGIC, SCALE_SUFFIX = 0x4C435345, ".embed_scale"
+
+
+def load_embed_scale(model_path: str) -> float:
+    """The factor on the embedding that the model was saved with."""
+    path = model_path + SCALE_SUFFIX
+    if not os.path.exists(path):
+        return 1.0
+    with open(path, "rb") as f:
+        raw = f.read()
+    if len(raw) != 12 or struct.unpack_from("<I", raw, 0)[0] != SCALE_MAGIC:
+        raise ValueError(f"{path}: not the embedding factor of a model")
+    return struct.unpack_from("<d", raw, 4)[0]
+
+
+def same_embed_scale(a: float, b: float) -> bool:
+    """Equal as the float32 numbers that the rows are multiplied with."""
+    return np.float32(a) == np.float32(b)
+
+
+def save_with_gains(path: str, m: Model, gains, embed_scale: float = 1.0) -> None:
+    """The model file and, beside it, its gains file and its embedding factor.  Without gains, or with a factor of 1, a file that an earlier model left there
+    goes: it would be read as this model's."""
     save(path, m)
     if gains:
         save_gains(path + GAINS_SUFFIX, gains)
     elif os.path.exists(path + GAINS_SUFFIX):
         os.remove(path + GAINS_SUFFIX)
+    if not same_embed_scale(embed_scale, 1.0):
+        with open(path + SCALE_SUFFIX, "wb") as f:
+            f.write(struct.pack("<Id", SCALE_MAGIC, embed_scale))
+    elif os.path.exists(path + SCALE_SUFFIX):
+        os.remove(path + SCALE_SUFFIX)
 
 
 def gain_names(n_layers: int):

@@ -868,7 +868,7 @@ def main(argv=None):
                     help="attention pairs that feed dK/dV: every descendant (default), the node's own query, or the queries on the key's radix edge")
     ap.add_argument("--group-rows", type=int, default=1_000_000)
     ap.add_argument("--qk-norm", action="store_true", help="RMS norm of queries and keys per head, with gains kept in a file beside the model's (MODEL.qk_gains)")
-    ap.add_argument("--embed-scale", type=float, default=1.0, help="factor on the embedding rows")
+    ap.add_argument("--embed-scale", type=float, default=1.0, help="factor on the embedding rows, kept in a file beside the model (MODEL.embed_scale); a model that has one takes no other")
     ap.add_argument("--activations-8bit", action="store_true",
                     help="keep the inputs of the q/k/v and feed-forward projections in 8 bits for the backward (less memory)")
     ap.add_argument("--ffn-recompute", action="store_true", help="recompute the FFN activations in the backward (less memory)")
@@ -884,6 +884,10 @@ def main(argv=None):
     args = ap.parse_args(argv)
     if args.activations_8bit and args.ffn_recompute:
         ap.error("--activations-8bit keeps what --ffn-recompute would form again: choose one")
+    if os.path.exists(args.model + MF.SCALE_SUFFIX):
+        trained_with = MF.load_embed_scale(args.model)
+        if not MF.same_embed_scale(args.embed_scale, trained_with):
+            raise SystemExit(f"{args.model} was trained with --embed-scale {trained_with!r}, not {args.embed_scale!r}")
 
     world, rank, local = (int(os.environ.get(k, d)) for k, d in (("WORLD_SIZE", "1"), ("RANK", "0"), ("LOCAL_RANK", "0")))
     if not torch.cuda.is_available():
@@ -940,9 +944,9 @@ def main(argv=None):
             print(f"Epoch {ep}: loss={ls / max(nq, 1):.6f}  ({time.time() - t0:.2f} sec, {units} subtrees, {chunks} chunks, {nq} nodes)",
                   flush=True)
             if args.save_every and ep % args.save_every == 0:
-                MF.save_with_gains(f"{save}.ep{ep}", model.to_model_file(), model.qk_gains())
+                MF.save_with_gains(f"{save}.ep{ep}", model.to_model_file(), model.qk_gains(), model.embed_scale)
     if rank == 0:
-        MF.save_with_gains(save, model.to_model_file(), model.qk_gains())
+        MF.save_with_gains(save, model.to_model_file(), model.qk_gains(), model.embed_scale)
     if world > 1:
         dist.destroy_process_group()
 
