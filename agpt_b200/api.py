@@ -902,7 +902,7 @@ def qk_norm_rope(q, k, q_gain, k_gain, pos, cos, sin, eps: float = 1e-6, k_dtype
     """Queries and keys with every head normalised by its root mean square (times a gain [head_dim], None: ones) and rotated by its row's
     position (as rope_pair_ does), in one pass.  q [n, heads * head_dim], k [n, kv_heads * head_dim], float32 or bfloat16, also as column
     ranges of one matrix; head_dim is the width of the tables.  k_dtype: torch.bfloat16 writes the keys as a bfloat16 store.  Outputs are new
-    tensors, or q_out and k_out (q and k themselves will do).  Returns (q, k)."""
+    tensors, or q_out and k_out (q and k themselves will do; one that overlaps the other side's rows is refused).  Returns (q, k)."""
     rt = _rt()
     kind, n, qc, q_ld, dev = _rows(rt, q, "q")
     kc = k.shape[-1]

@@ -721,6 +721,9 @@ extern "C" int agpt_b200_act8_relu_backward(const float *d_grad, int64_t ld, con
     if (ld < cols) return agpt_set_error(AGPT_E_ARG, "act8_relu_backward: bad stride");
     if (n == 0) return AGPT_OK;
     if (!d_grad || !d_out || !d_codes || !vec::aligned(d_codes, 16)) return agpt_set_error(AGPT_E_ARG, "act8_relu_backward: null or unaligned argument");
+    // where a row of grad lies elsewhere than the row of out, it could be written before it is read
+    if (!(d_out == d_grad && (ld == cols || n == 1)) && vec::overlap({d_out, (int64_t)cols * 4, (int64_t)cols * 4}, {d_grad, ld * 4, (int64_t)cols * 4}, n))
+        return agpt_set_error(AGPT_E_ARG, "act8_relu_backward: out overlaps grad and is not grad");
     const Shape s = shape_of(n, cols);
     const unsigned grid = (unsigned)((s.tasks + 31) / 32);
     const vec::Divide by(s.blocks);

@@ -405,6 +405,10 @@ int check(const char *who, int64_t n, int hq, int hk, int hd, int n_pos, int x_t
     return AGPT_OK;
 }
 
+// A head is read whole by the lanes that write it, so an output may lie on what its own side reads, row on row; on anything else it could be written before that is read.
+bool same_rows(const vec::Span &a, const vec::Span &b, int64_t n) { return a.p == b.p && a.width == b.width && (a.pitch == b.pitch || n == 1); }
+bool may_write(const vec::Span &out, const vec::Span &own, const vec::Span &other, int64_t n) { return (same_rows(out, own, n) || !vec::overlap(out, own, n)) && !vec::overlap(out, other, n); }
+
 }  // namespace
 
 extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void *d_k, int64_t k_ld, int type, const float *d_q_gain, const float *d_k_gain,
@@ -415,6 +419,10 @@ extern "C" int agpt_b200_qk_norm_rope(const void *d_q, int64_t q_ld, const void 
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad output type or stride");
     if (n == 0) return AGPT_OK;
     if (!d_q || !d_k || !d_pos || !d_cos || !d_sin || !d_q_out || !d_k_out) return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: bad argument");
+    const auto span = [&](const void *p, int64_t ld, int heads, int t) { return vec::Span{p, ld * bytes_of(t), (int64_t)heads * head_dim * bytes_of(t)}; };
+    const vec::Span q = span(d_q, q_ld, q_heads, type), k = span(d_k, k_ld, k_heads, type), qo = span(d_q_out, q_out_ld, q_heads, q_out_type), ko = span(d_k_out, k_out_ld, k_heads, k_out_type);
+    if (!may_write(qo, q, k, n) || !may_write(ko, k, q, n) || vec::overlap(qo, ko, n))
+        return agpt_set_error(AGPT_E_ARG, "qk_norm_rope: outputs overlap each other or inputs other than their own");
     Heads P{{d_q, nullptr, d_q_out, q_ld, 0, q_out_ld, d_q_gain, q_out_type == AGPT_KV_F32, q_heads, 0},
             {d_k, nullptr, d_k_out, k_ld, 0, k_out_ld, d_k_gain, k_out_type == AGPT_KV_F32, k_heads, 0},
             d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, 1.f / (float)head_dim, vec::Divide(1), nullptr, 0};
@@ -448,6 +456,11 @@ extern "C" int agpt_b200_qk_norm_rope_backward(const void *d_dq, int64_t dq_ld, 
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward: gain gradients overlap (one tensor for both, or two apart)");
     if (gains && (!d_workspace || workspace_bytes < agpt_b200_qk_norm_rope_backward_workspace_bytes(head_dim) || !vec::aligned(d_workspace, 16)))
         return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward: workspace too small (agpt_b200_qk_norm_rope_backward_workspace_bytes)");
+    const auto span = [&](const void *p, int64_t ld, int heads, int t) { return vec::Span{p, ld * bytes_of(t), (int64_t)heads * head_dim * bytes_of(t)}; };
+    const vec::Span q = span(d_q, q_ld, q_heads, type), k = span(d_k, k_ld, k_heads, type), qo = span(d_q_out, q_out_ld, q_heads, type), ko = span(d_k_out, k_out_ld, k_heads, type),
+                    dq = span(d_dq, dq_ld, q_heads, grad_type), dk = span(d_dk, dk_ld, k_heads, grad_type);
+    if (!may_write(qo, q, k, n) || !may_write(qo, dq, dk, n) || !may_write(ko, k, q, n) || !may_write(ko, dk, dq, n) || vec::overlap(qo, ko, n))
+        return agpt_set_error(AGPT_E_ARG, "qk_norm_rope_backward: outputs overlap each other or inputs other than their own");
     const int wide = type == AGPT_KV_F32, wide_dy = grad_type == AGPT_KV_F32;
     Heads P{{d_q, d_dq, d_q_out, q_ld, dq_ld, q_out_ld, d_q_gain, wide, q_heads, 0}, {d_k, d_dk, d_k_out, k_ld, dk_ld, k_out_ld, d_k_gain, wide, k_heads, 0},
             d_pos, d_cos, d_sin, n, head_dim, n_pos, 0, 0, eps, 1.f / (float)head_dim, vec::Divide(1), gains ? (float *)d_workspace : nullptr, 0};

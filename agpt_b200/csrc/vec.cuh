@@ -120,6 +120,17 @@ template <typename T, int VEC> struct Piece {
     }
 };
 
+// n rows of `width` bytes, `pitch` bytes apart: whether two such sets share bytes (of different pitches, whether their spans do)
+struct Span { const void *p; int64_t pitch, width; };
+inline bool overlap(Span a, Span b, int64_t n) {
+    int64_t between = (int64_t)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+    if (between < 0) { const Span t = a; a = b; b = t; between = -between; }
+    if (between >= (n - 1) * a.pitch + a.width) return false;
+    if (n == 1 || a.pitch != b.pitch) return true;
+    between %= a.pitch;
+    return between < a.width || between + b.width > a.pitch;
+}
+
 inline bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 // outputs larger than the caches: written past them

@@ -399,7 +399,7 @@ int64_t agpt_b200_embedding_grad_sorted_workspace_bytes(int64_t n, int d_model, 
 /* RMS norm per head of queries and keys with their rotation, in one pass:  y = R(pos) (gain * x / sqrt(mean(x^2) + eps))  for each of the q_heads
  * and k_heads heads of head_dim columns (even, up to 256), rotated as agpt_b200_rope does by tables [n_pos, head_dim] of cos and sin; a position outside the
  * tables takes the nearest row.  q and k: rows of `type`, their own strides (columns of one projection's output will do); outputs of any of the two types, so
- * that keys can go straight into a bfloat16 store; an output may be its input where types and strides are equal.  Gains [head_dim] float32, NULL: ones.
+ * that keys can go straight into a bfloat16 store; an output may be its input where types and strides are equal, and overlaps nothing else that is read or written (refused).  Gains [head_dim] float32, NULL: ones.
  * eps must be above 0.
  * Backward: from dq, dk of grad_type and the forward's inputs, the gradients with respect to q and k (of their type; may be written over dq and dk of that type
  * and stride).  Gain gradients [head_dim] float32 are accumulated into in a fixed order (NULL: not wanted; with both NULL no workspace is needed); one tensor for
