@@ -27,9 +27,6 @@ template <int VEC> __device__ __forceinline__ void load(const __nv_bfloat16 *p, 
         const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p));
         v[0] = low(x.x); v[1] = high(x.x); v[2] = low(x.y); v[3] = high(x.y);
         v[4] = low(x.z); v[5] = high(x.z); v[6] = low(x.w); v[7] = high(x.w);
-    } else if constexpr (VEC == 4) {
-        const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(p));
-        v[0] = low(x.x); v[1] = high(x.x); v[2] = low(x.y); v[3] = high(x.y);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; i++) v[i] = __bfloat162float(p[i]);
@@ -38,26 +35,6 @@ template <int VEC> __device__ __forceinline__ void load(const __nv_bfloat16 *p, 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
-}
-template <int VEC> __device__ __forceinline__ void store(float *p, const float (&v)[VEC]) {
-    if constexpr (VEC % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < VEC; i += 4) reinterpret_cast<float4 *>(p)[i / 4] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) p[i] = v[i];
-    }
-}
-// one rounding to bfloat16, to nearest, of the float32 result
-template <int VEC> __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
-    } else if constexpr (VEC == 4) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) p[i] = __float2bfloat16_rn(v[i]);
-    }
 }
 
 // The same in two steps, so that many loads are on their way before the first value is asked for: fetch() is one predicated load without a branch (zeros where it
@@ -133,16 +110,26 @@ inline bool overlap(Span a, Span b, int64_t n) {
 
 inline bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
-// outputs larger than the caches: written past them
+// outputs larger than the caches: whole pieces of 16 bytes are written past them
 template <int VEC> __device__ __forceinline__ void store_past(float *p, const float (&v)[VEC]) {
     if constexpr (VEC % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < VEC; i += 4) __stcs(reinterpret_cast<float4 *>(p) + i / 4, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-    } else store<VEC>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) p[i] = v[i];
+    }
 }
+// one rounding to bfloat16, to nearest, of the float32 result
 template <int VEC> __device__ __forceinline__ void store_past(__nv_bfloat16 *p, const float (&v)[VEC]) {
-    if constexpr (VEC == 8) __stcs(reinterpret_cast<uint4 *>(p), make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])));
-    else store<VEC>(p, v);
+    if constexpr (VEC == 8) {
+        __stcs(reinterpret_cast<uint4 *>(p), make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])));
+    } else if constexpr (VEC == 4) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) p[i] = __float2bfloat16_rn(v[i]);
+    }
 }
 
 // Division of 64-bit task numbers by a launch constant: the upper half of a product with ceil(2^64 / d), exact while task * d < 2^64
