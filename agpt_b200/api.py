@@ -967,7 +967,8 @@ def qk_norm_rope_backward(dq, dk, q, k, q_gain, k_gain, pos, cos, sin, dq_gain=N
 
 class Act8:
     """An activation [n, cols] kept in 8 bits: codes uint8 [n, cols rounded up to 32] (e4m3) and scales uint8 [blocks of 32 columns, n rounded up to 16];
-    the value of a code is the e4m3 number (codes 0x7f and 0xff: NaN) times 2^(scale - 127), a block of scale 255 is NaN (see agpt_b200_act8_pack)."""
+    the value of a code is the e4m3 number (codes 0x7f and 0xff: NaN) times 2^(scale - 127), a block of scale 255 is NaN (see agpt_b200_act8_pack).  act8_weight_grad
+    takes the values as bfloat16 numbers: exact for scales of 3 and more (act8_pack writes 17 at least)."""
 
     __slots__ = ("codes", "scales", "cols")
 

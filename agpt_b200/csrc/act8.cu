@@ -10,7 +10,8 @@
 //   codes  uint8 [rows][columns rounded up to 32] (zeros behind the last column)
 //   scales uint8 [blocks of 32 columns][rows rounded up to 16]
 //
-// Packing, unpacking and the ReLU's backward are bound by memory: 560k x 512 float32 209 us (6.9 TB/s) and 216 (6.7), 400k x 512 269 us (6.8).
+// Packing, unpacking and the ReLU's backward are bound by memory: 560k x 512 float32 209 us (6.9 TB/s) and 216 (6.7), 400k x 512 269 us (6.8).  Packing bfloat16 is half
+// arithmetic, 162 us (5.4 TB/s).  Rows of no whole 16-byte pieces, or off 16-byte boundaries, go element by element: 560k x 510 344 us, 256 and 408 (374 at 512); bfloat16 351.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
@@ -210,7 +211,8 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // memory: per 64 rows of 128 x 256 the raw rows in and out, the planes and the MMAs' reads of them, each plane of G against the same codes, move 224 KB, 1750 clocks at
 // 128 bytes, where the MMAs take 1536 and the memory 1100.  On the way here: accumulators drained every 64 rows by eight columns at a time 245 and 411 us, by TMA
 // and 16 columns 209 and 289, every 128 rows 155 and 222 (error 1e-7 to 3e-7), eight warps on X 157 and 178, both groups on each accumulator 139 and 177, all threads on
-// 128 columns of X 136 and 171.  Slower: stages of 32 rows (143 and 206), eight warps on G (146 and 207).
+// 128 columns of X 136 and 171.  Slower: stages of 32 rows (143 and 206), eight warps on G (146 and 207).  Later and on another GPU, where the same took 142 and 181: NaN codes 142 and
+// 184, infinite gradients 142 and 186.  Rows of G off 16-byte boundaries, 512 kept and 128: 178; 128 kept and 512: 328.
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
 constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, eight on the accumulators
 constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 8 * WG_ROWS, PLANE = WG_ROWS * WG_X * 2;
@@ -559,7 +561,8 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
 }
 
 // Sums of the slices in order.  A warp has 128 numbers; of many slices, the eight warps of a block have the same numbers and a run of the slices each.  The numbers are
-// the weight gradient's and, behind it, the bias gradient's.
+// the weight gradient's and, behind it, the bias gradient's.  Whole calls, split / not, us: 37 slices (3000 rows, 128 by 512) 10.7 / 22.0, 18 (20,000 rows, 512 by 512) 37.0 / 40.4,
+// 6 (1733 rows, 384 by 1536) 19.2 / 16.7.
 constexpr int SPLIT_FROM = 16;
 template <bool SPLIT>
 __global__ void __launch_bounds__(256) weight_finish_kernel(const float *__restrict__ part, const float *__restrict__ col_part, int slices, int64_t size, int cols,

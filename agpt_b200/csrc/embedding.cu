@@ -7,10 +7,14 @@
 // 8 bytes a row), pieces of the order are summed by warps, and what a token has in several pieces is added in the order of the pieces.  Up to 512 rows
 // need no order: the block of a token's first row looks for the others.
 //
-// Bound by memory where there are many columns: a gradient reads n rows once and writes the table once.  1.4M rows x 128 float32, 1000 tokens: lookup 108 us (6.7 TB/s
-// written), gradient 156 us, of which the sums 113 (6.4 TB/s read), the sort 28 and the joins 14; 65,537 x 1024 bfloat16, 50,021 tokens: 30 and 90 us (134 MB read, 205
-// written), sort 30.  Between a thousand and a hundred thousand rows the chain of short launches is what is left: 15 us at 600 x 128, 19 at 5000 x 256, 46 at 20,000 x 512
-// of 50,000 tokens (100 MB written).  Not kept: one cooperative launch with grid barriers for the whole sort (93 us where 90), pairs ordered in shared memory before they
+// Bound by memory where there are many columns: a gradient reads n rows once and writes the table once.  1.4M rows x 128 float32, 1000 tokens: lookup 108 us in a row of
+// lookups (6.6 TB/s written) and 130 between other calls, whose lines it first drives out of the L2; gradient 156 us, single launches by the profiler 30 for the sort, 112
+// for the sums (6.4 TB/s read) and 14 for the joins.  65,537 x 1024 bfloat16, 50,021 tokens: 30 and 88 us (134 MB read, 205 written); sort 30, sums 65, joins 7, which
+// overlap where each launch is placed early.  Between a thousand and a hundred thousand rows the chain of short launches is what is left: 15 us at 600 x 128, 19 at
+// 5000 x 256, 46 at 20,000 x 512 of 50,000 tokens (100 MB written).
+// Rows that are no whole 16-byte pieces, or off 16-byte boundaries, go element by element: 2.7M x 65 float32 329 and 976 us where 2.8M x 64 take 107 and 210, 1.4M x 128
+// off boundaries 670 (bfloat16: 309 and 1044, 77 and 253, 710).
+// Not kept: one cooperative launch with grid barriers for the whole sort (93 us where 90), pairs ordered in shared memory before they
 // are written (a pass of 1.4M rows 21 us where 17.5), pieces of eight bytes for narrow rows (52 us where 53 at 300,000 x 64).
 #include <cuda_runtime.h>
 
@@ -222,8 +226,12 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) move_kernel(const void *__res
 
 // ---- the same in one cluster: up to CLUSTER_ROWS rows -----------------------------------------------------------------------------
 // Eight blocks hold all pairs in shared memory and exchange counts and pairs there, digits of eight bits a pass.  Three launches a pass of a few microseconds each are
-// most of a gradient of so few rows (5000 rows of 10,000 tokens, 256 columns: 19 us, 24 by six launches; 600 of 1400, 128: 15 and 19 by calls, 16 and 27).  From some
-// 60,000 rows on eight SMs take longer than all of them: 23 us of 65,537 rows, six launches 27.
+// most of a gradient of so few rows (whole gradients, one cluster and launches per pass, us):
+//   tokens x columns           4096 rows       16,384        24,576        32,768        45,000        65,536
+//   200 x 64      (1 / 1 pass) 13.1 / 16.0   15.6 / 18.7   17.8 / 20.6   19.4 / 21.8   22.0 / 22.9   27.3 / 27.3
+//   1400 x 128    (2 / 1)      16.1 / 18.5   19.5 / 20.4   22.2 / 21.0   23.6 / 23.1   27.4 / 23.7   36.0 / 28.1
+//   50,000 x 256  (2 / 2)      24.0 / 31.0   27.6 / 34.3   30.7 / 36.7   34.2 / 38.8   41.4 / 42.7   50.1 / 49.2
+// So the limit is where the middle row has turned and the others have not; twice the rows would fit in shared memory, but eight SMs then take longer than all of them.
 constexpr int CLUSTER = 8, CLUSTER_WARPS = 32, CLUSTER_THREADS = CLUSTER_WARPS * 32, CLUSTER_BITS = 8, CLUSTER_BINS = 1 << CLUSTER_BITS;
 constexpr int CLUSTER_CHUNK = 4 * 1024, CLUSTER_ROWS = CLUSTER * CLUSTER_CHUNK;
 constexpr int CLUSTER_SMEM = 2 * CLUSTER_CHUNK * 8 + (CLUSTER_WARPS + 3) * CLUSTER_BINS * 4;
@@ -513,7 +521,8 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 4) sum_kernel(const T *__restr
 }
 
 // Tokens that began in a block of the sums and go on behind it: tail, then the heads of the blocks that begin with the token.  A warp has a block; where the heads
-// are many, all warps of the block come together and have a run of them each.
+// are many, all warps of the block come together and have a run of them each: from 17 on, 157 us at 1.4M x 128 of 1000 tokens and 168 of three; from 5 on 162 and 195, from 65
+// on 157 and 168 (25.2 where 23.8 at 40,000 x 256 of 40 tokens).
 constexpr int JOIN_ALONE = 16;
 template <typename O>
 __global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ order, int64_t n, int d, uint32_t vocab, int64_t span, int64_t blocks, float scale, int accumulate,
@@ -600,7 +609,9 @@ __global__ void __launch_bounds__(256) join_kernel(const uint2 *__restrict__ ord
 
 // ---- few rows: one launch, no order -------------------------------------------------------------------------------------------------
 // Every block reads all tokens; the block of a token's first row adds its rows, a run of the rows per warp; blocks behind fill absent tokens.
-constexpr int FEW_ROWS = 512;      // 5 us at 301 rows x 384, 1400 tokens; every block looks at all rows
+// Every block looks at all rows, so the work grows with their square, but up to the limit it is far below what the order costs (here / by the cluster, us): 256 rows x 384, 1400 tokens
+// 3.9 / 12.7, 512 4.7 / 13.1; 512 x 128 of 65 tokens 3.5 / 10.2.  1024 rows would still be ahead: 7.4 / 14.2 and 5.5 / 11.5.
+constexpr int FEW_ROWS = 512;
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(256) few_rows_kernel(const T *__restrict__ grad, int64_t ld, const void *__restrict__ ids, int wide, int n, int d, uint32_t vocab,
                                                         float scale, int accumulate, O *__restrict__ out) {

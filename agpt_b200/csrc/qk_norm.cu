@@ -336,6 +336,9 @@ bool type_ok(int t) { return t == AGPT_KV_F32 || t == AGPT_KV_BF16; }
 // every row of m starts on a boundary of `vec` elements of its type
 bool rows_aligned(const void *p, int64_t ld, int type, int vec) { return !p || (vec::aligned(p, vec * bytes_of(type) > 16 ? 16 : vec * bytes_of(type)) && ld % vec == 0); }
 
+// Heads of a group, whatever their number.  Many heads: four and two, 121 and 193 us at 400k rows of 4 + 4 x 32, 157 and 246 at 40k of 32 + 8 x 128 bfloat16; two and one 129 and
+// 228, 197 and 295; one in the forward 144 and 230, four in the backward 208 and 250.  Sides of one or two heads leave places of a group empty: 400k rows of 1 + 1 x 64 135 us, by one
+// head a group 76 (backward 143, 121); 200k of 2 + 2 x 64 83, by two 66 (103, by one 119).
 constexpr int HEADS = 4, BACK_HEADS = 2, MAX_HEADS = 1024;
 
 void split(Heads &P, int vec, int heads_each, int low) {

@@ -423,8 +423,8 @@ int64_t agpt_b200_qk_norm_rope_backward_workspace_bytes(int head_dim);
  *           both start on 16-byte boundaries
  * act8_pack: x of `type`, rows ld elements apart.  act8_unpack: the values, float32 [n, cols].  act8_relu_backward: out = grad where the kept activation is
  * above 0, else 0 (out contiguous, may be grad itself if that is).  act8_weight_grad: for kept inputs [n, m] of a projection and the gradient [n, cols] of its
- * output, weight_grad [m, cols] = X^T grad and bias_grad [cols] = column sums of grad (NULL: not wanted), float32-accurate over the kept values and repeatable
- * bit for bit. */
+ * output, weight_grad [m, cols] = X^T grad and bias_grad [cols] = column sums of grad (NULL: not wanted), float32-accurate over the kept values (which it takes
+ * as bfloat16 numbers: exact for scale bytes of 3 and more, pack writes 17 at least) and repeatable bit for bit. */
 int agpt_b200_act8_pack(const void *d_x, int64_t ld, int type, uint8_t *d_codes, uint8_t *d_scales, int64_t n, int cols, void *stream);
 int agpt_b200_act8_unpack(const uint8_t *d_codes, const uint8_t *d_scales, float *d_out, int64_t n, int cols, void *stream);
 int agpt_b200_act8_relu_backward(const float *d_grad, int64_t ld, const uint8_t *d_codes, float *d_out, int64_t n, int cols, void *stream);
