@@ -211,8 +211,9 @@ __global__ void __launch_bounds__(256) relu_backward_kernel(const float *grad, i
 // memory: per 64 rows of 128 x 256 the raw rows in and out, the planes and the MMAs' reads of them, each plane of G against the same codes, move 224 KB, 1750 clocks at
 // 128 bytes, where the MMAs take 1536 and the memory 1100.  On the way here: accumulators drained every 64 rows by eight columns at a time 245 and 411 us, by TMA
 // and 16 columns 209 and 289, every 128 rows 155 and 222 (error 1e-7 to 3e-7), eight warps on X 157 and 178, both groups on each accumulator 139 and 177, all threads on
-// 128 columns of X 136 and 171.  Slower: stages of 32 rows (143 and 206), eight warps on G (146 and 207).  Later and on another GPU, where the same took 142 and 181: NaN codes 142 and
-// 184, infinite gradients 142 and 186.  Rows of G off 16-byte boundaries, 512 kept and 128: 178; 128 kept and 512: 328.
+// 128 columns of X 136 and 171.  Slower: stages of 32 rows (143 and 206), eight warps on G (146 and 207).  Later, on another GPU and side by side, 128
+// kept and 512: 175 us as it was, 181 with NaN codes and infinite gradients, 183 with the bias gradient's blocks added in float64; 512 kept and 128: 140 to 142 throughout.
+// Rows of G off 16-byte boundaries, 512 kept and 128: 178; 128 kept and 512: 328.
 constexpr int WG_ROWS = 64, WG_X = 256, WG_G = 128, RAW_STAGES = 3;
 constexpr int WG_THREADS = 768;                        // four warps that load and issue MMAs, four on G, eight on X, eight on the accumulators
 constexpr uint32_t RAW_G = WG_ROWS * WG_G * 4, RAW_X = WG_ROWS * WG_X, RAW_S = 8 * WG_ROWS, PLANE = WG_ROWS * WG_X * 2;
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
             copies_end();
         };
         if (!TMA_G) { fetch(rb0, 0); fetch(rb0 + 1, 1); }
-        float csum = 0.f;
+        double csum = 0.;                                              // of row blocks, of which a slice may have thousands
         uint32_t i = 0, gp = 0;
         int slot = 0;
         for (int64_t rb = rb0; rb < rb1; rb++, i++) {
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(WG_THREADS, 1) weight_kernel(const __grid_cons
             if (++slot == RAW_STAGES) { slot = 0; gp ^= 1; }
         }
         if (!TMA_G) copies_wait<0>();
-        if (P.col_part && x0 == 0 && live) P.col_part[(int64_t)slice * P.cols + col] = csum;
+        if (P.col_part && x0 == 0 && live) P.col_part[(int64_t)slice * P.cols + col] = (float)csum;
     } else if (warp < 16) {
         regs_dec<REG_X>();
         // ---------------- X: a thread has 16 columns of four rows; of two where the block has up to 128 columns, since half of the
